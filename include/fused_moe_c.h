@@ -45,7 +45,7 @@ enum fmoe_status {
   FMOE_ERR_DEVICE_TIMEOUT = -5  /* a bounded device-side wait ran out (status word set) */
 };
 
-enum fmoe_dtype { FMOE_BF16 = 0, FMOE_FP8_E4M3 = 1 };
+enum fmoe_dtype { FMOE_BF16 = 0, FMOE_FP8_E4M3 = 1, FMOE_F16 = 2 /* grouped products and silu_mul only */ };
 
 enum fmoe_quant {
   FMOE_QUANT_NONE = 0,          /* bf16 activations and weights */
@@ -394,6 +394,50 @@ FMOE_API int fmoe_ep_wait_combine(const int32_t* topk_ids, int32_t T, int32_t K,
                                   const uint64_t* peer_base, const fmoe_ep_layout_c* lay, int32_t me, int32_t G,
                                   int32_t* epoch_dev, int32_t* scratch, void* out, int32_t* status,
                                   int32_t timeout_ms, void* stream);
+
+/* ---- Operators that an expert layer is built from when it is not one fmoe_run: training (with
+ * gradients), other activations, dense layers beside the experts.  Asynchronous on `stream`; no
+ * workspace, no device memory of their own, no host synchronisation; the same inputs give the same
+ * bits (no atomics).  Matrices are row-major and dense, 16-byte aligned.  `status` (optional) is a
+ * device int32 that receives a code if a bounded wait in a kernel runs out (the results are then
+ * not valid); it is not cleared.  No counterpart in the reference operator. */
+
+/* Products grouped by expert, ragged in the rows: group g owns the rows offsets[g] .. offsets[g+1]-1
+ * of the row matrices (offsets: device int32[groups + 1], read as a running maximum clamped to
+ * [0, rows], so any values are safe).  dtype: FMOE_BF16 or FMOE_F16; f32 sums, one rounding.
+ *   transpose_w = 0: out[r, :] = w[g] x[r, :]      x [rows, k] -> out [rows, n]
+ *   transpose_w = 1: out[r, :] = w[g]^T x[r, :]    x [rows, n] -> out [rows, k]  (gradient of x)
+ * w is [groups, n, k].  Rows of no group are zero.  n and k are multiples of 8, groups <= 1024. */
+FMOE_API int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* offsets, int64_t rows, int32_t groups,
+                                 int32_t n, int32_t k, int32_t dtype, int32_t transpose_w, void* out, int32_t* status,
+                                 void* stream);
+/* Gradient of w: dw[g] = sum over the rows r of group g of dy[r, :]^T x[r, :], dw [groups, n, k];
+ * zero for a group without rows.  Rows of no group do not enter it, whatever they hold. */
+FMOE_API int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const int32_t* offsets, int64_t rows, int32_t groups,
+                                       int32_t n, int32_t k, int32_t dtype, void* dw, int32_t* status, void* stream);
+
+/* Product of e4m3 matrices with a scale for each block of 128:
+ *   out[i, j] = bf16( sum_b a_scale[i, b] w_scale[j / 128, b] sum_{k in block b} a[i, k] w[j, k] )
+ * a [m, k] and a_scale as fmoe_quantise_rows writes them for `quant` (FMOE_QUANT_BLOCK128: f32
+ * [m, k/128]; FMOE_QUANT_BLOCK128_UE8M0: bytes [m, roundup(k/128, 4)]), w [n, k], w_scale f32
+ * [ceil(n/128), k/128] (powers of two for FMOE_QUANT_BLOCK128_UE8M0), out bf16 [m, n].  k is a
+ * multiple of 128, m and n are any. */
+FMOE_API int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
+                                  int32_t n, int32_t k, int32_t quant, void* out, int32_t* status, void* stream);
+
+/* The gated activation: out[r, i] = row_weight[r] * SiLU(gu[r, i]) * gu[r, width + i], gu [rows,
+ * 2*width] of dtype FMOE_BF16 or FMOE_F16 (gate columns, then up columns: the order of W1's rows),
+ * row_weight f32 [rows] or NULL (1).  f32 arithmetic, one rounding.  width is a multiple of 8. */
+FMOE_API int fmoe_silu_mul(const void* gu, const float* row_weight, int64_t rows, int32_t width, int32_t dtype, void* out,
+                           void* stream);
+/* The same rounded to dtype and then quantised to e4m3 with 1x128 scales, bit for bit what
+ * fmoe_quantise_rows makes of fmoe_silu_mul's bf16 result (quant: FMOE_QUANT_BLOCK128 or
+ * FMOE_QUANT_BLOCK128_UE8M0; width a multiple of 128). */
+FMOE_API int fmoe_silu_mul_quantise(const void* gu, const float* row_weight, int64_t rows, int32_t width, int32_t dtype,
+                                    int32_t quant, void* q, void* scales, void* stream);
+/* Gradients of fmoe_silu_mul: dgu [rows, 2*width] and, with row_weight, dweight f32 [rows]. */
+FMOE_API int fmoe_silu_mul_backward(const void* gu, const float* row_weight, const void* dy, int64_t rows, int32_t width,
+                                    int32_t dtype, void* dgu, float* dweight, void* stream);
 
 /* What one fmoe_run with these traits and dimensions will launch on the current device: the
  * kernel flavour of each GEMM (the same decision fmoe_run takes) and the number of kernels

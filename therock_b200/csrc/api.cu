@@ -2,7 +2,6 @@
 // sequence of the fused-MoE operator.  No device memory is allocated here; every buffer
 // belongs to the caller.
 #include <cuda_runtime.h>
-#include <nvtx3/nvToolsExt.h>
 
 #include <cstdio>
 #include <cstring>
@@ -10,47 +9,19 @@
 
 #include "../../include/fused_moe_c.h"
 #include "gemm.cuh"
+#include "host.cuh"
 #include "internal.h"
 #include "plan.hpp"
 
 namespace {
 
+using fmoe::DeviceGuard;
+using fmoe::NvtxRange;
 using fmoe::fail;
 using fmoe::Plan;
 using fmoe::make_plan;
 using fmoe::validate_dims;
 using fmoe::validate_traits;
-
-// Makes the device that owns `ptr` current for the lifetime of the object and puts the
-// caller's device back afterwards: the entry points leave no trace in the calling thread.
-class DeviceGuard {
- public:
-  explicit DeviceGuard(const void* ptr) {
-    cudaPointerAttributes attr;
-    if (ptr == nullptr || cudaPointerGetAttributes(&attr, ptr) != cudaSuccess) {
-      cudaGetLastError();   // not fatal: stay on the calling thread's device
-      return;
-    }
-    if (attr.type != cudaMemoryTypeDevice) return;
-    int cur = -1;
-    if (cudaGetDevice(&cur) != cudaSuccess || cur == attr.device) return;
-    if (cudaSetDevice(attr.device) != cudaSuccess) {
-      rc_ = fail(FMOE_ERR_CUDA, "cudaSetDevice(%d) failed", attr.device);
-      return;
-    }
-    prev_ = cur;
-  }
-  ~DeviceGuard() {
-    if (prev_ >= 0) cudaSetDevice(prev_);
-  }
-  DeviceGuard(const DeviceGuard&) = delete;
-  DeviceGuard& operator=(const DeviceGuard&) = delete;
-  int rc() const { return rc_; }
-
- private:
-  int prev_ = -1;
-  int rc_ = FMOE_OK;
-};
 
 // A pair of timing events that is destroyed on every exit path.
 struct EventPair {
@@ -60,19 +31,6 @@ struct EventPair {
     if (b) cudaEventDestroy(b);
   }
 };
-
-// NVTX range around one stage of the operator (a no-op unless a profiler is attached).
-struct NvtxRange {
-  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
-  ~NvtxRange() { nvtxRangePop(); }
-};
-
-#define FMOE_CUDA(expr)                                                                    \
-  do {                                                                                     \
-    cudaError_t e__ = (expr);                                                              \
-    if (e__ != cudaSuccess)                                                                \
-      return fail(FMOE_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__));         \
-  } while (0)
 
 }  // namespace
 

@@ -1,0 +1,311 @@
+// Product of e4m3 matrices with one scale per 128 of K on the activations' rows and per 128 x 128
+// block on the weights:
+//   out[i, j] = sum_b sa[i, b] sw[j / 128, b] P_b[i, j],   P_b = sum_{k in block b} a[i, k] w[j, k]
+//
+// The scales change with every block of K, so P_b is a fresh 128 x 256 accumulator in tensor memory
+// (one pipeline stage: 128 elements of K, four MMAs) and sixteen epilogue warps add it, scaled, to
+// running sums in registers: acc += P_b * (sa * sw), packed two at a time.  Warp (quadrant q, column
+// group c) owns rows 32q + lane and columns 64c .. 64c + 63, i.e. 64 sums a thread; four warps on
+// each scheduler take turns waiting for tensor memory and multiplying.  Two accumulators let the
+// MMAs of one stage run while the previous one is drained.
+//
+// A separate warp loads the scales of four blocks at a time, multiplies the activations' by the two
+// weight blocks' of the tile and leaves the products in shared memory, so the epilogue warps spend one
+// load on them.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "ptx.cuh"
+#include "scales.cuh"
+
+namespace fmoe {
+
+constexpr int kBmmThreads = 640;          // warps 0-3: TMA, MMA, scales, idle; warps 4-19: epilogue
+constexpr int kBmmEpiWarps = 16;
+constexpr int kBmmStages = 4;
+constexpr int kBmmTileM = 128, kBmmTileN = 256;
+constexpr int kBmmABytes = kBmmTileM * 128;
+constexpr int kBmmStageBytes = kBmmABytes + kBmmTileN * 128;
+constexpr int kBmmScaleSlots = 2;         // ring of scale products, four K blocks a slot
+constexpr int kBmmScaleSlotFloats = 4 * 2 * kBmmTileM;
+constexpr int kBmmEpiPitch = 12;          // words: 16 bf16 columns of a row, padded (conflict-free 16-byte accesses)
+constexpr int kBmmEpiBytes = kBmmEpiWarps * 32 * kBmmEpiPitch * 4;
+constexpr int kBmmMisc = 256;
+constexpr int kBmmSmemBytes = kBmmStages * kBmmStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
+static_assert(kBmmSmemBytes <= 227 * 1024, "shared memory budget");
+// setmaxnreg redistributes the 640 x 96 registers of the launch: what the roles take must not exceed it.
+constexpr int kBmmThinRegs = 64, kBmmFatRegs = 104;
+static_assert(128 * kBmmThinRegs + 512 * kBmmFatRegs <= kBmmThreads * 96, "register budget");
+
+enum : int { kStatusBmmTimeout = 0x600 };
+
+struct BlockMatmulParams {
+  const void* a_scale;      // f32 [m, kb] or UE8M0 bytes [m, scale_pitch(kb)]
+  const float* w_scale;     // [ceil(n / 128), kb]
+  int m, n, kb;             // kb: blocks of 128 along K
+  int m_blocks, n_blocks;   // tiles
+  __nv_bfloat16* out;
+  int* status;              // may be null
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ void bmm_fail(int* status, int code) {
+  if (status != nullptr) atomicExch(status, kStatusBmmTimeout | code);
+}
+
+// Exponent byte -> power of two (0 is 2^-127, 255 is NaN).
+__device__ __forceinline__ float ue8m0_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : (byte == 255u ? 0x7fffffffu : byte << 23));
+}
+
+template <bool kBytes>
+__global__ void __launch_bounds__(kBmmThreads, 1)
+fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                            const BlockMatmulParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* misc = smem + kBmmStages * kBmmStageBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(misc);
+  uint64_t* empty_bar = full_bar + kBmmStages;
+  uint64_t* part_full_bar = empty_bar + kBmmStages;      // [2]
+  uint64_t* part_empty_bar = part_full_bar + 2;          // [2]
+  uint64_t* sc_full_bar = part_empty_bar + 2;            // [kBmmScaleSlots]
+  uint64_t* sc_empty_bar = sc_full_bar + kBmmScaleSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty_bar + kBmmScaleSlots);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* sc_ring = reinterpret_cast<float*>(misc + kBmmMisc);
+  uint32_t* epi = reinterpret_cast<uint32_t*>(sc_ring + kBmmScaleSlots * kBmmScaleSlotFloats);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tm_a);
+    ptx::prefetch_tensormap(&tm_w);
+    for (int i = 0; i < kBmmStages; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(ptx::smem_u32(&part_full_bar[b]), 1);
+      ptx::mbar_init(ptx::smem_u32(&part_empty_bar[b]), kBmmEpiWarps);
+    }
+    for (int i = 0; i < kBmmScaleSlots; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&sc_full_bar[i]), 32);
+      ptx::mbar_init(ptx::smem_u32(&sc_empty_bar[i]), kBmmEpiWarps);
+    }
+    *abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::pdl_wait();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total_tiles = p.m_blocks * p.n_blocks;
+
+  if (warp < 4) {
+    ptx::setmaxnreg_dec<kBmmThinRegs>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+        const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
+        for (int k = 0; k < p.kb; ++k) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+          const uint32_t full = ptx::smem_u32(&full_bar[stage]);
+          const uint32_t sa = ptx::smem_u32(smem + stage * kBmmStageBytes);
+          ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
+          ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
+          ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+          if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) bmm_fail(p.status, 0x01);
+      ptx::pdl_release();
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------------- MMA issuer
+      constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
+      int stage = 0;
+      uint32_t phase = 0;
+      int buf = 0;
+      uint32_t buf_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+        for (int k = 0; k < p.kb; ++k) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&part_empty_bar[buf]), buf_phase ^ 1u, abort_flag) ||
+              !ptx::mbar_wait(ptx::smem_u32(&full_bar[stage]), phase, abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * kBmmTileN);
+          const uint32_t sa = ptx::smem_u32(smem + stage * kBmmStageBytes);
+          const uint64_t da = ptx::make_smem_desc(kDesc, sa);
+          const uint64_t db = ptx::make_smem_desc(kDesc, sa + kBmmABytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
+          ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
+          ptx::umma_commit(ptx::smem_u32(&part_full_bar[buf]));
+          if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
+          if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
+        }
+      }
+      if (!ok) bmm_fail(p.status, 0x02);
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- scale products
+      int slot = 0;
+      uint32_t sphase = 0;
+      bool ok = true;
+      const int nb = (p.n + 127) >> 7;
+      const int pitch = scale_pitch(p.kb);
+      const bool vec = kBytes || ((p.kb & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0);
+      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+        const int m0 = tile % p.m_blocks * kBmmTileM, nb0 = tile / p.m_blocks * 2;
+        const float* sw0 = p.w_scale + static_cast<size_t>(nb0) * p.kb;
+        const float* sw1 = p.w_scale + static_cast<size_t>(min(nb0 + 1, nb - 1)) * p.kb;
+        for (int k = 0; k < p.kb; k += 4) {
+          float w0[4], w1[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w0[j] = k + j < p.kb ? __ldg(sw0 + k + j) : 0.0f;
+            w1[j] = k + j < p.kb ? __ldg(sw1 + k + j) : 0.0f;
+          }
+          float s[4][4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = m0 + 32 * r + lane;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[r][j] = 0.0f;
+            if (row < p.m) {
+              if (kBytes) {
+                const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(row) * pitch + k));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[r][j] = ue8m0_value((b >> (8 * j)) & 0xffu);
+              } else {
+                const float* src = static_cast<const float*>(p.a_scale) + static_cast<size_t>(row) * p.kb + k;
+                if (vec) {
+                  const float4 v = __ldg(reinterpret_cast<const float4*>(src));
+                  s[r][0] = v.x; s[r][1] = v.y; s[r][2] = v.z; s[r][3] = v.w;
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    if (k + j < p.kb) s[r][j] = __ldg(src + j);
+                }
+              }
+            }
+          }
+          if (!ptx::mbar_wait(ptx::smem_u32(&sc_empty_bar[slot]), sphase ^ 1u, abort_flag)) { ok = false; break; }
+          float* dst = sc_ring + slot * kBmmScaleSlotFloats;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              dst[(2 * j) * kBmmTileM + 32 * r + lane] = s[r][j] * w0[j];
+              dst[(2 * j + 1) * kBmmTileM + 32 * r + lane] = s[r][j] * w1[j];
+            }
+          ptx::mbar_arrive(ptx::smem_u32(&sc_full_bar[slot]));
+          if (++slot == kBmmScaleSlots) { slot = 0; sphase ^= 1u; }
+        }
+      }
+      if (!ok && lane == 0) bmm_fail(p.status, 0x03);
+    }
+  } else {
+    // ------------------------------------------------------------------ promotion and epilogue
+    ptx::setmaxnreg_inc<kBmmFatRegs>();
+    const int quad = warp & 3;
+    const int cg = (warp - 4) >> 2;                      // 64-column group
+    uint32_t* mine = epi + (warp - 4) * (32 * kBmmEpiPitch);
+    int buf = 0, slot = 0;
+    uint32_t buf_phase = 0, sphase = 0;
+    bool ok = true;
+    const bool vec_out = (p.n & 7) == 0;
+    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
+      uint64_t acc[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) acc[j] = 0ull;
+      for (int k = 0; k < p.kb; ++k) {
+        if ((k & 3) == 0 && !ptx::mbar_wait(ptx::smem_u32(&sc_full_bar[slot]), sphase, abort_flag)) { ok = false; break; }
+        const float sc = sc_ring[slot * kBmmScaleSlotFloats + (2 * (k & 3) + (cg >> 1)) * kBmmTileM + quad * 32 + lane];
+        const uint64_t sc2 = ptx::pack2(sc, sc);
+        if (!ptx::mbar_wait(ptx::smem_u32(&part_full_bar[buf]), buf_phase, abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        const uint32_t t = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(buf * kBmmTileN + cg * 64);
+        uint32_t v[2][16];
+        ptx::tmem_ld_32x16(t, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ptx::tmem_ld_wait();
+          if (c < 3) ptx::tmem_ld_32x16(t + (c + 1) * 16, v[(c + 1) & 1]);
+          if (c == 3) {
+            // everything has left this accumulator: the MMAs may overwrite it
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&part_empty_bar[buf]));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ptx::fma2(acc[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], sc2);
+        }
+        if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
+        if ((k & 3) == 3 || k + 1 == p.kb) {
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sc_empty_bar[slot]));
+          if (++slot == kBmmScaleSlots) { slot = 0; sphase ^= 1u; }
+        }
+      }
+      if (!ok) break;
+      // one rounding to bf16; 16 columns at a time turn through shared memory so that two lanes write
+      // 32 consecutive bytes of a row
+      const int row0 = m0 + quad * 32;
+      const int col0 = n0 + cg * 64;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float lo, hi;
+          ptx::unpack2(acc[c * 8 + j], lo, hi);
+          const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+          w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        __syncwarp();
+        uint4* dst = reinterpret_cast<uint4*>(mine + lane * kBmmEpiPitch);
+        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int r = it * 16 + (lane >> 1);
+          const int col = col0 + c * 16 + (lane & 1) * 8;
+          if (row0 + r < p.m && col < p.n) {
+            const uint4 val = *reinterpret_cast<const uint4*>(mine + r * kBmmEpiPitch + (lane & 1) * 4);
+            __nv_bfloat16* o = p.out + static_cast<size_t>(row0 + r) * p.n + col;
+            if (vec_out) {
+              *reinterpret_cast<uint4*>(o) = val;
+            } else {
+              const uint32_t x[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (col + e < p.n) reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+        }
+      }
+    }
+    if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x04);
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace fmoe

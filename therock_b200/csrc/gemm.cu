@@ -32,6 +32,16 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// The encoder needs a context on the calling thread, which a thread that has made no other runtime
+// call yet (an autograd worker, for one) does not have: selecting its device makes the context current.
+template <typename Encode>
+CUresult with_context(Encode encode) {
+  CUresult r = encode();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  return r;
+}
+
 // Row-major [rows, k_elems] matrix, box = 128 bytes of K x box_rows rows, 128-byte swizzle.
 CUresult make_map(CUtensorMap* tm, const void* base, bool fp8, int64_t rows, int k_elems,
                   int box_rows = kSlabRows) {
@@ -42,10 +52,12 @@ CUresult make_map(CUtensorMap* tm, const void* base, bool fp8, int64_t rows, int
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(k_elems) * esize};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(kStageKBytes / esize), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  return fn(tm, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return with_context([&] {
+    return fn(tm, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 constexpr int kMaxDevices = 64;
@@ -99,6 +111,20 @@ cudaError_t launch_pair_variant(const CUtensorMap& ta, const CUtensorMap& tb, co
 }
 
 }  // namespace
+
+CUresult encode_tensor_map(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                           const uint64_t* stride_bytes, const uint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return CUDA_ERROR_NOT_FOUND;
+  const cuuint32_t estr[3] = {1, 1, 1};
+  cuuint64_t d[3], st[2];
+  cuuint32_t b[3];
+  for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i + 1 < rank) st[i] = stride_bytes[i]; }
+  return with_context([&] {
+    return fn(tm, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
 
 // A library built with -DFMOE_TIMING_SWITCHES honours FMOE_GEMM_MODE=1cta / 2cta, which forces one
 // kernel flavour for every GEMM (used to compare them); the product build ignores the variable.

@@ -1,0 +1,525 @@
+// Products grouped by expert for sm_100a, ragged in the rows, as operators with gradients.
+//
+//   rows kernel   out[r, :] = W_g x[r, :]   (kWMnMajor = false: W [G, N, K], contraction over K)
+//                 out[r, :] = W_g^T x[r, :] (kWMnMajor = true: contraction over N; W is read as it
+//                                            lies, the MMA takes it MN-major)
+//   wgrad kernel  dW_g = sum_r dy[r, :]^T x[r, :], both operands MN-major, contraction over the
+//                 group's rows
+//
+// Both are persistent kernels of CTA pairs (cta_group::2, 256 x 256 tiles, 64 elements of the
+// contraction per stage, six stages, two 256-column accumulators in tensor memory), with the roles
+// of the pair kernel of the fused operator: producer warp, MMA warp, four epilogue warps.
+//
+// Rows kernel: the weights are the MMA's M side and the rows its N side.  M tiles of weights are
+// always full, and N goes in steps of 32, so a group of any size costs its own rows rounded up to
+// 32 instead of to 256.  A group of s rows is cut into ceil(s / 256) chunks of equal size.
+// Rows of a neighbouring group that come along in the last 32 only produce accumulator columns
+// that nobody stores.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace fmoe {
+
+constexpr int kGrpThreads = 192;
+constexpr int kGrpMaxGroups = 1024;
+constexpr int kGrpStages = 6;
+constexpr int kGrpOperandBytes = 128 * 128;                 // 128 rows (or two 64-column chunks x 64 rows) x 128 bytes
+constexpr int kGrpStageBytes = 2 * kGrpOperandBytes;
+constexpr int kGrpStageK = 64;                              // 16-bit elements of the contraction per stage
+constexpr int kGrpTile = 256;
+constexpr int kGrpMisc = 256 + 2 * (kGrpMaxGroups + 8) * 4; // barriers, group starts, cumulative chunks
+constexpr int kGrpStageWords = 20;                          // row pitch of a warp's transpose area, in words
+constexpr int kGrpEpiBytes = 4 * 32 * kGrpStageWords * 4;
+constexpr int kGrpSmemBytes = kGrpStages * kGrpStageBytes + kGrpMisc + kGrpEpiBytes + 1024;
+static_assert(kGrpSmemBytes <= 227 * 1024, "shared memory budget");
+
+enum : int { kStatusGroupedTimeout = 0x500 };
+
+struct GroupedParams {
+  const int32_t* offsets;   // [groups + 1]
+  int groups;
+  int rows;
+  int m_blocks;             // rows kernel: 256-wide blocks of output columns; wgrad: blocks of N
+  int k_blocks;             // wgrad: 256-wide blocks of K
+  int k_iters;              // rows kernel: stages per tile
+  int n, k;                 // wgrad: dimensions of dw; rows kernel: n = output columns
+  uint16_t* out;
+  int* status;              // may be null
+  uint32_t idesc;           // instruction descriptor without N (rows kernel) / complete (wgrad)
+};
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if (kBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void grouped_fail(const GroupedParams& p, int code) {
+  if (p.status != nullptr) atomicExch(p.status, kStatusGroupedTimeout | code);
+}
+
+// One warp: starts[0 .. G] = running maximum of the offsets clamped to [0, rows];
+// cum[0 .. G] = cumulative number of `chunk`-row pieces.
+__device__ __forceinline__ void scan_groups(const int32_t* offsets, int groups, int rows, int chunk, int* starts, int* cum) {
+  const int lane = threadIdx.x & 31;
+  int run_start = min(max(offsets[0], 0), rows), run_cum = 0;
+  if (lane == 0) { starts[0] = run_start; cum[0] = 0; }
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int end = g < groups ? min(max(offsets[g + 1], 0), rows) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end = max(end, o);
+    }
+    end = max(end, run_start);
+    int start = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) start = run_start;
+    int c = g < groups ? (end - start + chunk - 1) / chunk : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, c, d);
+      if (lane >= d) c += o;
+    }
+    c += run_cum;
+    if (g < groups) { starts[g + 1] = end; cum[g + 1] = c; }
+    run_start = __shfl_sync(0xffffffffu, end, 31);
+    run_cum = __shfl_sync(0xffffffffu, c, 31);
+  }
+}
+
+struct RowsTile {
+  int group, m_blk;
+  int row0, live;           // first row of the chunk, rows of it
+  int n;                    // MMA columns: live rounded up to 32
+};
+
+// Tile order: group, then block of output columns, then the group's chunks: CTA pairs that run
+// side by side read the same weights, once from memory and then from L2.
+__device__ __forceinline__ RowsTile decode_rows_tile(int tile, const int* starts, const int* cum, int groups, int m_blocks) {
+  int lo = 1, hi = groups;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (static_cast<long long>(cum[mid]) * m_blocks > tile) hi = mid; else lo = mid + 1;
+  }
+  RowsTile t;
+  t.group = lo - 1;
+  const int cnt = cum[lo] - cum[lo - 1];
+  const int local = tile - cum[lo - 1] * m_blocks;
+  t.m_blk = local / cnt;
+  const int chunk = local % cnt;
+  const int size = starts[lo] - starts[lo - 1];
+  // equal chunks in steps of 32; the last one is never empty (fewer than 32 * cnt rows are lost to
+  // the rounding, and only where cnt < 8, since the chunks are 256 long otherwise)
+  const int per = ((size + cnt - 1) / cnt + 31) & ~31;
+  t.row0 = starts[lo - 1] + chunk * per;
+  t.live = min(per, size - chunk * per);
+  t.n = (t.live + 31) & ~31;
+  return t;
+}
+
+struct GroupedSmem {
+  uint8_t* stages;
+  uint64_t *full_bar, *empty_bar, *acc_full_bar, *acc_empty_bar, *tail_bar;
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+  int *starts, *cum;
+  uint32_t* epi;
+};
+__device__ __forceinline__ GroupedSmem carve_grouped_smem(uint8_t* raw) {
+  GroupedSmem s;
+  s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* misc = s.stages + kGrpStages * kGrpStageBytes;
+  s.full_bar = reinterpret_cast<uint64_t*>(misc);       // used in rank 0
+  s.empty_bar = s.full_bar + kGrpStages;                // both ranks
+  s.acc_full_bar = s.empty_bar + kGrpStages;            // [2] both ranks
+  s.acc_empty_bar = s.acc_full_bar + 2;                 // [2] used in rank 0
+  s.tail_bar = s.acc_empty_bar + 2;                     // wgrad: ragged last stage of this CTA
+  s.tmem_slot = reinterpret_cast<uint32_t*>(s.tail_bar + 1);
+  s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
+  s.starts = reinterpret_cast<int*>(misc + 256);
+  s.cum = s.starts + kGrpMaxGroups + 8;
+  s.epi = reinterpret_cast<uint32_t*>(misc + kGrpMisc);
+  return s;
+}
+
+// Barriers, tensor memory, group table.  `full_count`: arrivals per stage besides the bytes.
+__device__ __forceinline__ uint32_t grouped_setup(const GroupedSmem& s, const GroupedParams& p, int full_count, int warp) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kGrpStages; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&s.full_bar[i]), full_count);
+      ptx::mbar_init(ptx::smem_u32(&s.empty_bar[i]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(ptx::smem_u32(&s.acc_full_bar[b]), 1);
+      ptx::mbar_init(ptx::smem_u32(&s.acc_empty_bar[b]), 8);      // 4 epilogue warps in each CTA
+    }
+    ptx::mbar_init(ptx::smem_u32(s.tail_bar), 1);
+    *s.abort_flag = 0;
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(s.tmem_slot), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::pdl_wait();              // the offsets and operands of this call are read from here on
+  if (warp == 2) scan_groups(p.offsets, p.groups, p.rows, kGrpTile, s.starts, s.cum);
+  ptx::tc_fence_before();
+  ptx::cluster_sync_all();      // both CTAs' barriers are initialised before anyone signals them
+  ptx::tc_fence_after();
+  return *s.tmem_slot;
+}
+
+__device__ __forceinline__ void grouped_teardown(uint32_t tmem_base, int warp) {
+  // neither CTA leaves while its partner can still signal its barriers or read its shared memory
+  ptx::tc_fence_before();
+  ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// Tensor maps of the row matrix with boxes of 128, 64, 32 and 16 rows: a chunk's half, a multiple
+// of 16 up to 128, is the sum of at most four of them.
+struct RowMaps {
+  CUtensorMap m[4];
+};
+
+template <bool kBf16, bool kWMnMajor>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGrpThreads, 1)
+fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ RowMaps tm_x,
+                         const GroupedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const GroupedSmem s = carve_grouped_smem(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tm_w);
+    for (int i = 0; i < 4; ++i) ptx::prefetch_tensormap(&tm_x.m[i]);
+  }
+  const uint32_t tmem_base = grouped_setup(s, p, 1, warp);
+  const int total_tiles = s.cum[p.groups] * p.m_blocks;
+  const int first_tile = blockIdx.x >> 1;
+  const int tile_step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both ranks)
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
+        const int m0 = t.m_blk * kGrpTile + static_cast<int>(rank) * 128;
+        const int half = t.n >> 1;
+        const int r0 = t.row0 + static_cast<int>(rank) * half;
+        const uint32_t bytes = 2u * (kGrpOperandBytes + half * 128);
+        for (int k = 0; k < p.k_iters; ++k) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&s.empty_bar[stage]), phase ^ 1u, s.abort_flag)) { ok = false; break; }
+          // completion bytes of both CTAs are credited to rank 0's barrier
+          const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(&s.full_bar[stage]), 0);
+          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
+          const uint32_t sb = sa + kGrpOperandBytes;
+          if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&s.full_bar[stage]), bytes);
+          const int kx = k * kGrpStageK;
+          if (kWMnMajor) {
+            ptx::tma_load_3d_pair(sa, &tm_w, full0, m0, kx, t.group);
+            ptx::tma_load_3d_pair(sa + kGrpOperandBytes / 2, &tm_w, full0, m0 + 64, kx, t.group);
+          } else {
+            ptx::tma_load_3d_pair(sa, &tm_w, full0, kx, m0, t.group);
+          }
+          int done = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int box = 128 >> i;
+            if (half & box) {
+              ptx::tma_load_2d_pair(sb + done * 128, &tm_x.m[i], full0, kx, r0 + done);
+              done += box;
+            }
+          }
+          if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) grouped_fail(p, 0x01);
+      ptx::pdl_release();   // all operands requested: the next kernel may begin its set-up
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (rank 0 only)
+    if (lane == 0 && rank == 0) {
+      constexpr uint64_t kDescA = kWMnMajor ? ptx::sw128_mnmajor_desc_template(kGrpOperandBytes / 2)
+                                            : ptx::sw128_kmajor_desc_template();
+      constexpr uint64_t kDescB = ptx::sw128_kmajor_desc_template();
+      // 16 elements of the contraction: 32 bytes along a swizzled row, or 16 rows of 128 bytes
+      constexpr uint64_t kAdvA = kWMnMajor ? (16 * 128) >> 4 : 32 >> 4;
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
+        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(t.n >> 3) << 17);
+        if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_empty_bar[acc]), acc_phase ^ 1u, s.abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGrpTile);
+        for (int k = 0; k < p.k_iters; ++k) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&s.full_bar[stage]), phase, s.abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
+          const uint64_t da = ptx::make_smem_desc(kDescA, sa);
+          const uint64_t db = ptx::make_smem_desc(kDescB, sa + kGrpOperandBytes);
+#pragma unroll
+          for (int kk = 0; kk < kGrpStageK / 16; ++kk)
+            ptx::umma_f16_pair(d_tmem, da + kk * kAdvA, db + kk * 2, idesc, (k | kk) ? 1u : 0u);
+          const uint32_t e_local = ptx::smem_u32(&s.empty_bar[stage]);
+          ptx::umma_commit_pair(e_local);
+          ptx::umma_commit_pair(ptx::map_to_rank(e_local, 1));
+          if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        const uint32_t f_local = ptx::smem_u32(&s.acc_full_bar[acc]);
+        ptx::umma_commit_pair(f_local);
+        ptx::umma_commit_pair(ptx::map_to_rank(f_local, 1));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+      if (!ok) grouped_fail(p, 0x02);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue warps (both ranks)
+    // Lane = output column, accumulator column = row of the result: two lanes swap halves of a
+    // packed pair so that every lane stores two neighbouring columns of one row.
+    const int quad = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
+      if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag)) { ok = false; break; }
+      ptx::tc_fence_after();
+      const int col = t.m_blk * kGrpTile + static_cast<int>(rank) * 128 + quad * 32 + (lane & ~1);
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);
+      uint16_t* o = p.out + static_cast<size_t>(t.row0 + (lane & 1)) * p.n + col;
+      for (int c = 0; c < t.live; c += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(t_addr + c, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const uint32_t mine = pack16<kBf16>(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+          // even lane: row j, columns (lane, lane + 1); odd lane: row j + 1, columns (lane - 1, lane)
+          const uint32_t word = (lane & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+          if (col < p.n && c + j + (lane & 1) < t.live)
+            *reinterpret_cast<uint32_t*>(o + static_cast<size_t>(c + j) * p.n) = word;
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && threadIdx.x == 64) grouped_fail(p, 0x03);
+    // rows of no group: in front of the first one and behind the last
+    const int head = s.starts[0], tail = s.starts[p.groups];
+    const int vecs = p.n >> 3;
+    const long long total = static_cast<long long>(head + p.rows - tail) * vecs;
+    for (long long i = static_cast<long long>(blockIdx.x) * 128 + (threadIdx.x - 64); i < total; i += static_cast<long long>(gridDim.x) * 128) {
+      long long r = i / vecs;
+      const int v = static_cast<int>(i - r * vecs);
+      if (r >= head) r += tail - head;
+      *reinterpret_cast<uint4*>(p.out + static_cast<size_t>(r) * p.n + v * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  grouped_teardown(tmem_base, warp);
+}
+
+// dW_g [N, K] in 256 x 256 tiles.  The contraction runs over the group's rows, 64 per stage and 16
+// per MMA, from the group's first row on (a TMA box may start at any row).  The last stage issues
+// only the MMAs it has rows for; where the last 16 are not full, the rest of them holds rows of the
+// next group (or whatever lies behind the last one, which may be infinite or NaN), so both CTAs'
+// producer warps overwrite those rows with zeros before the MMA may read them.
+template <bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGrpThreads, 1)
+fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
+                          const GroupedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const GroupedSmem s = carve_grouped_smem(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tm_dy);
+    ptx::prefetch_tensormap(&tm_x);
+  }
+  const uint32_t tmem_base = grouped_setup(s, p, 2, warp);
+  const int per_group = p.m_blocks * p.k_blocks;
+  const int total_tiles = p.groups * per_group;
+  const int first_tile = blockIdx.x >> 1;
+  const int tile_step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both ranks)
+    int stage = 0;
+    uint32_t phase = 0, tail_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const int g = tile / per_group;
+      const int local = tile - g * per_group;
+      const int n0 = local / p.k_blocks * kGrpTile + static_cast<int>(rank) * 128;
+      const int k0 = local % p.k_blocks * kGrpTile + static_cast<int>(rank) * 128;
+      const int row0 = s.starts[g];
+      const int size = s.starts[g + 1] - row0;
+      for (int done = 0; done < size; done += kGrpStageK) {
+        if (!ptx::mbar_wait(ptx::smem_u32(&s.empty_bar[stage]), phase ^ 1u, s.abort_flag)) { ok = false; break; }
+        const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(&s.full_bar[stage]), 0);
+        const int live = min(kGrpStageK, size - done);
+        const bool ragged = (live & 15) != 0;
+        uint8_t* st = s.stages + stage * kGrpStageBytes;
+        const uint32_t sa = ptx::smem_u32(st);
+        if (lane == 0) {
+          uint32_t bar = full0;
+          if (ragged) {
+            // the bytes of this CTA are waited for here; rank 0's barrier then gets one arrival from each CTA
+            bar = ptx::map_to_rank(ptx::smem_u32(s.tail_bar), rank);
+            ptx::mbar_arrive_expect_tx(ptx::smem_u32(s.tail_bar), kGrpStageBytes);
+          } else if (rank == 0) {
+            ptx::mbar_arrive_expect_tx(ptx::smem_u32(&s.full_bar[stage]), 2 * kGrpStageBytes);
+          } else {
+            ptx::mbar_arrive_cluster(full0);
+          }
+          const int r = row0 + done;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            ptx::tma_load_2d_pair(sa + c * (kGrpOperandBytes / 2), &tm_dy, bar, n0 + 64 * c, r);
+            ptx::tma_load_2d_pair(sa + kGrpOperandBytes + c * (kGrpOperandBytes / 2), &tm_x, bar, k0 + 64 * c, r);
+          }
+        }
+        if (ragged) {
+          __syncwarp();
+          if (!ptx::mbar_wait(ptx::smem_u32(s.tail_bar), tail_phase, s.abort_flag)) { ok = false; break; }
+          tail_phase ^= 1u;
+          const int last = (live + 15) & ~15;
+          // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
+          for (int i = lane; i < (last - live) * 32; i += 32) {
+            const int row = live + (i >> 5);
+            const int c = (i >> 3) & 3;
+            *reinterpret_cast<uint4*>(st + c * (kGrpOperandBytes / 2) + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(full0);
+        }
+        if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) grouped_fail(p, 0x11);
+    if (lane == 0) ptx::pdl_release();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (rank 0 only)
+    if (lane == 0 && rank == 0) {
+      constexpr uint64_t kDesc = ptx::sw128_mnmajor_desc_template(kGrpOperandBytes / 2);
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        const int g = tile / per_group;
+        const int size = s.starts[g + 1] - s.starts[g];
+        if (size == 0) continue;
+        if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_empty_bar[acc]), acc_phase ^ 1u, s.abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGrpTile);
+        for (int done = 0; done < size; done += kGrpStageK) {
+          if (!ptx::mbar_wait_cluster(ptx::smem_u32(&s.full_bar[stage]), phase, s.abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
+          const uint64_t da = ptx::make_smem_desc(kDesc, sa);
+          const uint64_t db = ptx::make_smem_desc(kDesc, sa + kGrpOperandBytes);
+          const int steps = (min(kGrpStageK, size - done) + 15) >> 4;
+          for (int kk = 0; kk < steps; ++kk)
+            ptx::umma_f16_pair(d_tmem, da + kk * 128, db + kk * 128, p.idesc, (done | kk) ? 1u : 0u);
+          const uint32_t e_local = ptx::smem_u32(&s.empty_bar[stage]);
+          ptx::umma_commit_pair(e_local);
+          ptx::umma_commit_pair(ptx::map_to_rank(e_local, 1));
+          if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        const uint32_t f_local = ptx::smem_u32(&s.acc_full_bar[acc]);
+        ptx::umma_commit_pair(f_local);
+        ptx::umma_commit_pair(ptx::map_to_rank(f_local, 1));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+      if (!ok) grouped_fail(p, 0x12);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue warps (both ranks)
+    const int quad = warp & 3;
+    uint32_t* stage_w = s.epi + quad * (32 * kGrpStageWords);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const int g = tile / per_group;
+      const int local = tile - g * per_group;
+      const int n0 = local / p.k_blocks * kGrpTile + static_cast<int>(rank) * 128 + quad * 32;
+      const int k0 = local % p.k_blocks * kGrpTile;
+      const bool empty = s.starts[g + 1] == s.starts[g];
+      if (!empty) {
+        if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+      }
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);
+      uint16_t* o = p.out + (static_cast<size_t>(g) * p.n + n0) * p.k + k0;
+      const int cols = min(kGrpTile, p.k - k0);
+      for (int c = 0; c < cols; c += 32) {
+        uint32_t v[32];
+        if (!empty) {
+          ptx::tmem_ld_32x32(t_addr + c, v);
+          ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0u;
+        }
+        uint4* mine = reinterpret_cast<uint4*>(stage_w + lane * kGrpStageWords);
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          mine[q] = make_uint4(pack16<kBf16>(__uint_as_float(v[8 * q]), __uint_as_float(v[8 * q + 1])),
+                               pack16<kBf16>(__uint_as_float(v[8 * q + 2]), __uint_as_float(v[8 * q + 3])),
+                               pack16<kBf16>(__uint_as_float(v[8 * q + 4]), __uint_as_float(v[8 * q + 5])),
+                               pack16<kBf16>(__uint_as_float(v[8 * q + 6]), __uint_as_float(v[8 * q + 7])));
+        __syncwarp();
+        // 4 lanes per row, 8 rows per store instruction: 64 contiguous bytes per row
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (lane >> 2);
+          const int seg = (lane & 3) * 8;
+          if (n0 + r < p.n && c + seg < cols)
+            *reinterpret_cast<uint4*>(o + static_cast<size_t>(r) * p.k + c + seg) =
+                *reinterpret_cast<const uint4*>(stage_w + r * kGrpStageWords + seg / 2);
+        }
+      }
+      if (empty) continue;
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (!ok && threadIdx.x == 64) grouped_fail(p, 0x13);
+  }
+  grouped_teardown(tmem_base, warp);
+}
+
+}  // namespace fmoe

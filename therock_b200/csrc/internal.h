@@ -1,6 +1,7 @@
 // Launchers shared between the translation units of libfmoe_b200.so (not part of the ABI).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -114,6 +115,11 @@ struct GemmLaunch {
 // Returns cudaSuccess or the failing CUDA error; *drv_err receives a CUresult when the
 // tensor-map encode fails.
 cudaError_t launch_grouped_gemm(const GemmLaunch& g, cudaStream_t stream, int* drv_err);
+
+// Tensor map of a row-major array (dims and box innermost first, strides of the outer dimensions in
+// bytes, rank 2 or 3) read in 128-byte-swizzled boxes; what lies outside is filled with zeros.
+CUresult encode_tensor_map(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                           const uint64_t* stride_bytes, const uint32_t* box);
 
 // 0 = no override; 1 / 2 force the single-CTA / CTA-pair kernel.  Always 0 unless the library
 // was built with -DFMOE_TIMING_SWITCHES (then FMOE_GEMM_MODE=1cta|2cta is honoured).

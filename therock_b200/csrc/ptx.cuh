@@ -86,6 +86,17 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
+// 3-D tiled load, completion on an mbarrier of this CTA.
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* tm, uint32_t bar, int32_t x, int32_t y,
+                                            int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 // Release fence at system scope (the acquire/release form, not the sequentially consistent
 // membar.sys that __threadfence_system() emits): with a relaxed system-scope store after it this
 // is a release that is cumulative over everything the thread has observed.
@@ -228,6 +239,45 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtens
       : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar_cluster_addr), "r"(x), "r"(y)
       : "memory");
 }
+// The same in three dimensions.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtensorMap* tm, uint32_t bar_cluster_addr,
+                                                 int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// mbar_wait that also acquires what a thread of the peer CTA released with its arrival.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (!mbar_try_wait_cluster(bar, parity)) {
+    if ((++spins & 0xFFu) == 0) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kWaitLimitCycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result),
                "r"(ncols)
@@ -308,6 +358,13 @@ __host__ __device__ constexpr uint64_t sw128_kmajor_desc_template() {
        | (static_cast<uint64_t>(1) << 46)             // version
        | (static_cast<uint64_t>(2) << 61);            // SWIZZLE_128B
 }
+// The same for an MN-major tile: rows of the matrix in memory run along K, 64 16-bit elements of
+// M (or N) to a 128-byte swizzled row.  Eight K rows are 1024 bytes (stride byte offset); the next
+// 64 elements of M are `chunk_bytes` away (leading byte offset).
+__host__ __device__ constexpr uint64_t sw128_mnmajor_desc_template(uint32_t chunk_bytes) {
+  return (static_cast<uint64_t>(chunk_bytes >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
 __device__ __forceinline__ uint64_t make_smem_desc(uint64_t desc_template, uint32_t smem_addr) {
   return desc_template | static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);  // 16-byte units
 }
@@ -334,6 +391,10 @@ __device__ __forceinline__ uint32_t idesc_with_scale_byte(uint32_t idesc, uint32
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t fmt_ab, uint32_t m, uint32_t n) {
   return (1u << 4) | (fmt_ab << 7) | (fmt_ab << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
+
+// Bits of the instruction descriptor that mark A / B as MN-major.
+constexpr uint32_t kIdescAMnMajor = 1u << 15;
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
 
 }  // namespace ptx
 }  // namespace fmoe

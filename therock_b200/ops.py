@@ -1,0 +1,323 @@
+"""Operators an expert layer is built from when it is not one fused call.
+
+    grouped_matmul(x, weight, offsets)             rows grouped by expert times that expert's weight
+    matmul_block128(a, a_scale, w, w_scale, quant) e4m3 matrices with a scale for each block of 128
+    silu_mul(gu, row_weight)                       the gated activation, optionally times a weight per row
+    silu_mul_quantise(gu, quant, row_weight)       the same as e4m3 rows with their scales
+
+`grouped_matmul` and `silu_mul` have gradients (first order, through torch.autograd).  Every call
+enqueues kernels of libfmoe_b200.so on `stream` (the tensors' current stream by default) and
+returns: no host synchronisation, no atomics, so the same inputs give the same bits, and a call can
+be captured in a CUDA graph.  Inputs are contiguous CUDA tensors on one device, which need not be
+the current one; a call on another stream than the current one allocates its results for that
+stream, and the caller orders the streams.  Bad arguments raise FmoeError before any launch."""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .api import QUANT, FmoeError, _check, lib
+
+_DTYPE = {torch.bfloat16: 0, torch.float16: 2}
+_E4M3 = (torch.float8_e4m3fn, torch.uint8)
+_BLOCK_QUANT = ("block128", "block128_ue8m0")
+
+
+def _bound():
+    """The library with the signatures of these entry points set."""
+    l = lib()
+    if l.fmoe_grouped_matmul.argtypes is None:
+        vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+        l.fmoe_grouped_matmul_wgrad.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, vp]
+        l.fmoe_matmul_block128.argtypes = [vp, vp, vp, vp, i64, i32, i32, i32, vp, vp, vp]
+        l.fmoe_silu_mul.argtypes = [vp, vp, i64, i32, i32, vp, vp]
+        l.fmoe_silu_mul_quantise.argtypes = [vp, vp, i64, i32, i32, i32, vp, vp, vp]
+        l.fmoe_silu_mul_backward.argtypes = [vp, vp, vp, i64, i32, i32, vp, vp, vp]
+        l.fmoe_grouped_matmul.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp]
+    return l
+
+
+# One status word per device, made at the first call outside a stream capture (a tensor allocated
+# inside one would belong to that graph).  Kernels only write to it when a bounded wait runs out.
+_status: dict = {}
+
+
+def _status_ptr(device: torch.device) -> Optional[int]:
+    t = _status.get(device.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        with torch.cuda.device(device):
+            t = torch.zeros(1, dtype=torch.int32, device=device)
+            torch.cuda.current_stream(device).synchronize()   # the word is zero before any stream's kernel may set it
+        _status[device.index] = t
+    return t.data_ptr()
+
+
+def operator_status(device=None) -> int:
+    """Waits for the device and returns the code of the last bounded wait that ran out in one of this
+    module's kernels (0: none did), and clears it."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    t = _status.get(device.index)
+    if t is None:
+        return 0
+    torch.cuda.synchronize(device)
+    code = int(t.item())
+    if code:
+        t.zero_()
+    return code
+
+
+def _stream_of(t: torch.Tensor, stream) -> int:
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _empty(shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
+    """A result, allocated for the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=like.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _dense(name: str, t, device=None, align: int = 16) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous()):
+        raise FmoeError(-1, f"{name} must be a contiguous CUDA tensor")
+    if t.data_ptr() % align:
+        raise FmoeError(-1, f"{name} must be {align}-byte aligned")
+    if device is not None and t.device != device:
+        raise FmoeError(-1, f"{name} is on {t.device}, the other tensors on {device}")
+
+
+def _result(name: str, out, shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
+    if out is None:
+        return _empty(shape, dtype, like, stream)
+    _dense(name, out, like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise FmoeError(-1, f"{name} must be {dtype} {tuple(shape)}")
+    return out
+
+
+def _for_kernel(t: torch.Tensor) -> torch.Tensor:
+    """A gradient that autograd may hand over with any strides (expanded, sliced) as the kernels read it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+# ----------------------------------------------------------------------------- products grouped by expert
+def _check_grouped(x, weight, offsets):
+    _dense("x", x)
+    _dense("weight", weight, x.device)
+    _dense("offsets", offsets, x.device, 4)
+    if x.dtype not in _DTYPE or weight.dtype != x.dtype:
+        raise FmoeError(-1, "x and weight must both be bfloat16 or both float16")
+    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
+        raise FmoeError(-1, "x must be [rows, k] and weight [groups, n, k]")
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
+        raise FmoeError(-1, "offsets must be int32 [groups + 1]")
+
+
+def _grouped(x, weight, offsets, transpose: bool, out, stream):
+    groups, n, k = weight.shape
+    out = _result("out", out, (x.shape[0], k if transpose else n), x.dtype, x, stream)
+    _check(_bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
+                                        _DTYPE[x.dtype], int(transpose), out.data_ptr(), _status_ptr(x.device),
+                                        _stream_of(x, stream)))
+    return out
+
+
+def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                         stream=None) -> torch.Tensor:
+    """dx [rows, k] with dx[r] = weight[g]^T dy[r] for the rows of group g, zeros for rows of none: the
+    gradient of grouped_matmul with respect to x, from dy [rows, n]."""
+    _dense("dy", dy)
+    _dense("weight", weight, dy.device)
+    _dense("offsets", offsets, dy.device, 4)
+    if dy.dtype not in _DTYPE or weight.dtype != dy.dtype:
+        raise FmoeError(-1, "dy and weight must both be bfloat16 or both float16")
+    if dy.dim() != 2 or weight.dim() != 3 or weight.shape[1] != dy.shape[1]:
+        raise FmoeError(-1, "dy must be [rows, n] and weight [groups, n, k]")
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
+        raise FmoeError(-1, "offsets must be int32 [groups + 1]")
+    return _grouped(dy, weight, offsets, True, out, stream)
+
+
+def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                         stream=None) -> torch.Tensor:
+    """dw [groups, n, k] with dw[g] = dy[rows of g]^T x[rows of g]; zeros for a group without rows.
+    Rows of no group do not enter it, whatever they hold."""
+    _dense("dy", dy)
+    _dense("x", x, dy.device)
+    _dense("offsets", offsets, dy.device, 4)
+    if x.dtype not in _DTYPE or dy.dtype != x.dtype:
+        raise FmoeError(-1, "dy and x must both be bfloat16 or both float16")
+    if x.dim() != 2 or dy.dim() != 2 or x.shape[0] != dy.shape[0]:
+        raise FmoeError(-1, "dy must be [rows, n] and x [rows, k]")
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise FmoeError(-1, "offsets must be int32 [groups + 1]")
+    groups, n, k = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
+    out = _result("out", out, (groups, n, k), x.dtype, x, stream)
+    _check(_bound().fmoe_grouped_matmul_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
+                                              _DTYPE[x.dtype], out.data_ptr(), _status_ptr(x.device), _stream_of(x, stream)))
+    return out
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        ctx.save_for_backward(x, weight, offsets)
+        return _grouped(x, weight, offsets, False, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, offsets = ctx.saved_tensors
+        dy = _for_kernel(dy)
+        dx = grouped_matmul_dgrad(dy, weight, offsets) if ctx.needs_input_grad[0] else None
+        dw = grouped_matmul_wgrad(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                   stream=None) -> torch.Tensor:
+    """y[r] = weight[g] @ x[r] for the rows offsets[g] <= r < offsets[g + 1] of group g.
+
+    x [rows, k] and weight [groups, n, k] (the library's order: output channels, then k contiguous),
+    both bfloat16 or both float16; offsets int32 [groups + 1] on the device, so routing needs no host
+    step.  Sums are 32-bit, rounded once.  Groups may be empty; rows of no group (before offsets[0],
+    from offsets[-1] on) give zero rows and zero gradients.  Offsets are read as a running maximum
+    clamped to [0, rows].  n and k are multiples of 8, at most 1024 groups.  Differentiable in x and
+    weight; `out` and `stream` are for calls without gradients."""
+    _check_grouped(x, weight, offsets)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        if out is not None or stream is not None:
+            raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
+        return _GroupedMatmul.apply(x, weight, offsets)
+    return _grouped(x, weight, offsets, False, out, stream)
+
+
+# ----------------------------------------------------------------------------- e4m3 products with block scales
+def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, quant: str = "block128",
+                    out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """bf16 [m, n] = (a * its scales) @ (w * its scales)^T, one scale per 128 of k.
+
+    a [m, k] e4m3 (float8_e4m3fn, or its bytes as uint8) and a_scale as `quantise_rows(x, quant)`
+    returns them, or a_scale as float32 [m, k/128] for "block128"; w [n, k] e4m3 and w_scale float32
+    [ceil(n/128), k/128] (powers of two for "block128_ue8m0").  Each block's products are summed in 32
+    bits and scaled by both scales before blocks are added, in 32 bits; one rounding.  k is a multiple
+    of 128, m and n are any."""
+    if quant not in _BLOCK_QUANT:
+        raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
+    _dense("a", a)
+    _dense("w", w, a.device)
+    if a.dtype not in _E4M3 or w.dtype not in _E4M3:
+        raise FmoeError(-1, "a and w must be float8_e4m3fn (or uint8 holding it)")
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise FmoeError(-1, "a must be [m, k] and w [n, k]")
+    m, k = a.shape
+    n = w.shape[0]
+    if k % 128:
+        raise FmoeError(-2, "k must be a multiple of 128")
+    blocks = k // 128
+    row_bytes = 4 * blocks if quant == "block128" else (blocks + 3) // 4 * 4
+    _dense("a_scale", a_scale, a.device, 4)
+    _dense("w_scale", w_scale, a.device, 4)
+    if a_scale.dtype not in ((torch.float32, torch.uint8) if quant == "block128" else (torch.uint8,)) or \
+            tuple(a_scale.shape) != (m, row_bytes // a_scale.element_size()):
+        raise FmoeError(-1, f"a_scale must hold {row_bytes} bytes for each of the {m} rows, as quantise_rows returns them")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != ((n + 127) // 128, blocks):
+        raise FmoeError(-1, f"w_scale must be float32 [{(n + 127) // 128}, {blocks}]")
+    out = _result("out", out, (m, n), torch.bfloat16, a, stream)
+    _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
+                                         QUANT[quant], out.data_ptr(), _status_ptr(a.device), _stream_of(a, stream)))
+    return out
+
+
+# ----------------------------------------------------------------------------- the gated activation
+def _check_silu(gu, row_weight):
+    _dense("gu", gu)
+    if gu.dtype not in _DTYPE:
+        raise FmoeError(-1, "gu must be bfloat16 or float16")
+    if gu.dim() != 2 or gu.shape[1] % 2:
+        raise FmoeError(-1, "gu must be [rows, 2 * width]")
+    if row_weight is not None:
+        _dense("row_weight", row_weight, gu.device, 4)
+        if row_weight.dtype != torch.float32 or tuple(row_weight.shape) != (gu.shape[0],):
+            raise FmoeError(-1, "row_weight must be float32 [rows]")
+    return gu.shape[0], gu.shape[1] // 2
+
+
+def _silu(gu, row_weight, out, stream):
+    rows, width = gu.shape[0], gu.shape[1] // 2
+    out = _result("out", out, (rows, width), gu.dtype, gu, stream)
+    _check(_bound().fmoe_silu_mul(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
+                                  _DTYPE[gu.dtype], out.data_ptr(), _stream_of(gu, stream)))
+    return out
+
+
+def silu_mul_backward(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optional[torch.Tensor] = None, stream=None):
+    """Gradients of silu_mul: (dgu [rows, 2 * width], dweight float32 [rows] or None)."""
+    rows, width = _check_silu(gu, row_weight)
+    _dense("dy", dy, gu.device)
+    if dy.dtype != gu.dtype or tuple(dy.shape) != (rows, width):
+        raise FmoeError(-1, "dy must be [rows, width] of gu's type")
+    dgu = _empty((rows, 2 * width), gu.dtype, gu, stream)
+    dweight = None if row_weight is None else _empty((rows,), torch.float32, gu, stream)
+    _check(_bound().fmoe_silu_mul_backward(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), dy.data_ptr(),
+                                           rows, width, _DTYPE[gu.dtype], dgu.data_ptr(),
+                                           None if dweight is None else dweight.data_ptr(), _stream_of(gu, stream)))
+    return dgu, dweight
+
+
+class _SiluMul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gu, row_weight):
+        ctx.save_for_backward(gu, row_weight)
+        return _silu(gu, row_weight, None, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        gu, row_weight = ctx.saved_tensors
+        return silu_mul_backward(gu, _for_kernel(dy), row_weight)
+
+
+def silu_mul(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+             stream=None) -> torch.Tensor:
+    """out[r, i] = row_weight[r] * SiLU(gu[r, i]) * gu[r, width + i] for gu [rows, 2 * width] in
+    bfloat16 or float16 (gate columns, then up columns), row_weight float32 [rows] or none.  32-bit
+    arithmetic, one rounding; width is a multiple of 8.  Differentiable in gu and row_weight; `out`
+    and `stream` are for calls without gradients."""
+    _check_silu(gu, row_weight)
+    if torch.is_grad_enabled() and (gu.requires_grad or (row_weight is not None and row_weight.requires_grad)):
+        if out is not None or stream is not None:
+            raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
+        return _SiluMul.apply(gu, row_weight)
+    return _silu(gu, row_weight, out, stream)
+
+
+def silu_mul_quantise(gu: torch.Tensor, quant: str, row_weight: Optional[torch.Tensor] = None,
+                      q: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, stream=None):
+    """quantise_rows(silu_mul(gu, row_weight), quant) in one pass, bit for bit, for the block modes:
+    (q uint8 [rows, width], scales uint8 [rows, bytes]).  width is a multiple of 128.  No gradient."""
+    if quant not in _BLOCK_QUANT:
+        raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
+    rows, width = _check_silu(gu, row_weight)
+    if width % 128:
+        raise FmoeError(-2, "width must be a multiple of 128")
+    groups = width // 128
+    row_bytes = 4 * groups if quant == "block128" else (groups + 3) // 4 * 4
+    q = _result("q", q, (rows, width), torch.uint8, gu, stream)
+    scales = _result("scales", scales, (rows, row_bytes), torch.uint8, gu, stream)
+    _check(_bound().fmoe_silu_mul_quantise(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
+                                           _DTYPE[gu.dtype], QUANT[quant], q.data_ptr(), scales.data_ptr(),
+                                           _stream_of(gu, stream)))
+    return q, scales
