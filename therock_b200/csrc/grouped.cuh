@@ -201,7 +201,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                          const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
   const GroupedSmem s = carve_grouped_smem(smem_raw);
-  const int warp = threadIdx.x >> 5;
+  const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   if (threadIdx.x == 0) {
@@ -215,53 +215,62 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both ranks)
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
-        const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
-        const int m0 = t.m_blk * kGrpTile + static_cast<int>(rank) * 128;
-        const int half = t.n >> 1;
-        const int r0 = t.row0 + static_cast<int>(rank) * half;
-        const uint32_t bytes = 2u * (kGrpOperandBytes + half * 128);
-        for (int k = 0; k < p.k_iters; ++k) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&s.empty_bar[stage]), phase ^ 1u, s.abort_flag)) { ok = false; break; }
-          // completion bytes of both CTAs are credited to rank 0's barrier
-          const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(&s.full_bar[stage]), 0);
-          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
-          const uint32_t sb = sa + kGrpOperandBytes;
-          if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&s.full_bar[stage]), bytes);
+    const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(s.full_bar), 0);   // completion bytes of both CTAs go to rank 0
+    const uint32_t full_own = ptx::smem_u32(s.full_bar), empty_own = ptx::smem_u32(s.empty_bar);
+    const uint32_t smem0 = ptx::smem_u32(s.stages);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
+      const int group = ptx::uniform(t.group);
+      const int m0 = ptx::uniform(t.m_blk) * kGrpTile + static_cast<int>(rank) * 128;
+      const int half = ptx::uniform(t.n) >> 1;
+      const int r0 = ptx::uniform(t.row0) + static_cast<int>(rank) * half;
+      const uint32_t bytes = 2u * (kGrpOperandBytes + half * 128);
+      for (int k = 0; k < p.k_iters; ++k) {
+        if (!ptx::mbar_wait(empty_own + 8 * stage, phase ^ 1u, s.abort_flag)) { ok = false; break; }
+        if (ptx::elect_one()) {
+          const uint32_t full = full0 + 8 * stage;
+          const uint32_t sa = smem0 + stage * kGrpStageBytes;
           const int kx = k * kGrpStageK;
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full_own + 8 * stage, bytes);
           if (kWMnMajor) {
-            ptx::tma_load_3d_pair(sa, &tm_w, full0, m0, kx, t.group);
-            ptx::tma_load_3d_pair(sa + kGrpOperandBytes / 2, &tm_w, full0, m0 + 64, kx, t.group);
+            ptx::tma_load_3d_pair(sa, &tm_w, full, m0, kx, group);
+            ptx::tma_load_3d_pair(sa + kGrpOperandBytes / 2, &tm_w, full, m0 + 64, kx, group);
           } else {
-            ptx::tma_load_3d_pair(sa, &tm_w, full0, kx, m0, t.group);
+            ptx::tma_load_3d_pair(sa, &tm_w, full, kx, m0, group);
           }
           int done = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int box = 128 >> i;
             if (half & box) {
-              ptx::tma_load_2d_pair(sb + done * 128, &tm_x.m[i], full0, kx, r0 + done);
+              ptx::tma_load_2d_pair(sa + kGrpOperandBytes + done * 128, &tm_x.m[i], full, kx, r0 + done);
               done += box;
             }
           }
-          if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
       }
-      if (!ok) grouped_fail(p, 0x01);
-      ptx::pdl_release();   // all operands requested: the next kernel may begin its set-up
     }
+    if (!ok && lane == 0) grouped_fail(p, 0x01);
+    ptx::pdl_release();   // all operands requested: the next kernel may begin its set-up
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (rank 0 only)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint64_t kDescA = kWMnMajor ? ptx::sw128_mnmajor_desc_template(kGrpOperandBytes / 2)
                                             : ptx::sw128_kmajor_desc_template();
       constexpr uint64_t kDescB = ptx::sw128_kmajor_desc_template();
       // 16 elements of the contraction: 32 bytes along a swizzled row, or 16 rows of 128 bytes
       constexpr uint64_t kAdvA = kWMnMajor ? (16 * 128) >> 4 : 32 >> 4;
+      const uint32_t smem0 = ptx::smem_u32(s.stages);
+      const uint64_t da0 = ptx::make_smem_desc(kDescA, smem0);
+      const uint64_t db0 = ptx::make_smem_desc(kDescB, smem0 + kGrpOperandBytes);
+      const uint32_t full_own = ptx::smem_u32(s.full_bar), empty_own = ptx::smem_u32(s.empty_bar);
+      const uint32_t empty_peer = ptx::map_to_rank(empty_own, 1);
+      const uint32_t acc_full = ptx::smem_u32(s.acc_full_bar), acc_full_peer = ptx::map_to_rank(acc_full, 1);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -269,31 +278,34 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
       bool ok = true;
       for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
         const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
-        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(t.n >> 3) << 17);
+        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(ptx::uniform(t.n) >> 3) << 17);
         if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_empty_bar[acc]), acc_phase ^ 1u, s.abort_flag)) { ok = false; break; }
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGrpTile);
         for (int k = 0; k < p.k_iters; ++k) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&s.full_bar[stage]), phase, s.abort_flag)) { ok = false; break; }
+          if (!ptx::mbar_wait(full_own + 8 * stage, phase, s.abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
-          const uint64_t da = ptx::make_smem_desc(kDescA, sa);
-          const uint64_t db = ptx::make_smem_desc(kDescB, sa + kGrpOperandBytes);
+          if (ptx::elect_one()) {
+            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kGrpStageBytes >> 4));
+            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kGrpStageBytes >> 4));
 #pragma unroll
-          for (int kk = 0; kk < kGrpStageK / 16; ++kk)
-            ptx::umma_f16_pair(d_tmem, da + kk * kAdvA, db + kk * 2, idesc, (k | kk) ? 1u : 0u);
-          const uint32_t e_local = ptx::smem_u32(&s.empty_bar[stage]);
-          ptx::umma_commit_pair(e_local);
-          ptx::umma_commit_pair(ptx::map_to_rank(e_local, 1));
+            for (int kk = 0; kk < kGrpStageK / 16; ++kk)
+              ptx::umma_f16_pair(d_tmem, da + kk * kAdvA, db + kk * 2, idesc, (k | kk) ? 1u : 0u);
+            ptx::umma_commit_pair(empty_own + 8 * stage);
+            ptx::umma_commit_pair(empty_peer + 8 * stage);
+          }
+          __syncwarp();
           if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        const uint32_t f_local = ptx::smem_u32(&s.acc_full_bar[acc]);
-        ptx::umma_commit_pair(f_local);
-        ptx::umma_commit_pair(ptx::map_to_rank(f_local, 1));
+        if (ptx::elect_one()) {
+          ptx::umma_commit_pair(acc_full + 8 * acc);
+          ptx::umma_commit_pair(acc_full_peer + 8 * acc);
+        }
+        __syncwarp();
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok) grouped_fail(p, 0x02);
+      if (!ok && lane == 0) grouped_fail(p, 0x02);
     }
   } else {
     // ------------------------------------------------------------------ epilogue warps (both ranks)
@@ -310,19 +322,38 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
       const int col = t.m_blk * kGrpTile + static_cast<int>(rank) * 128 + quad * 32 + (lane & ~1);
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);
       uint16_t* o = p.out + static_cast<size_t>(t.row0 + (lane & 1)) * p.n + col;
-      for (int c = 0; c < t.live; c += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(t_addr + c, v);
+      const size_t step = 2 * static_cast<size_t>(p.n);
+      uint32_t v[2][32];
+      ptx::tmem_ld_32x32(t_addr, v[0]);
+      auto block = [&](uint32_t (&cur)[32], uint32_t (&next)[32], int c) {
         ptx::tmem_ld_wait();
+        if (c + 32 < t.live) ptx::tmem_ld_32x32(t_addr + c + 32, next);
+        uint32_t word[16];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const uint32_t mine = pack16<kBf16>(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t mine = pack16<kBf16>(__uint_as_float(cur[2 * j]), __uint_as_float(cur[2 * j + 1]));
           const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-          // even lane: row j, columns (lane, lane + 1); odd lane: row j + 1, columns (lane - 1, lane)
-          const uint32_t word = (lane & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-          if (col < p.n && c + j + (lane & 1) < t.live)
-            *reinterpret_cast<uint32_t*>(o + static_cast<size_t>(c + j) * p.n) = word;
+          // even lane: row 2j, columns (lane, lane + 1); odd lane: row 2j + 1, columns (lane - 1, lane)
+          word[j] = (lane & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
         }
+        // one branch for the whole block: a branch per store left the shuffles unoverlapped (a
+        // 256-column tile took 8.3 us, as long as 20 stages of MMAs)
+        if (col < p.n) {
+          if (c + 32 <= t.live) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) *reinterpret_cast<uint32_t*>(o + j * step) = word[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c + 2 * j + (lane & 1) < t.live) *reinterpret_cast<uint32_t*>(o + j * step) = word[j];
+          }
+        }
+        __syncwarp();
+        o += 16 * step;
+      };
+      for (int c = 0; c < t.live; c += 64) {
+        block(v[0], v[1], c);
+        if (c + 32 < t.live) block(v[1], v[0], c + 32);
       }
       ptx::tc_fence_before();
       __syncwarp();
@@ -355,7 +386,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
                           const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
   const GroupedSmem s = carve_grouped_smem(smem_raw);
-  const int warp = threadIdx.x >> 5;
+  const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   if (threadIdx.x == 0) {
@@ -370,6 +401,10 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both ranks)
+    const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(s.full_bar), 0);
+    const uint32_t full_own = ptx::smem_u32(s.full_bar), empty_own = ptx::smem_u32(s.empty_bar);
+    const uint32_t tail_own = ptx::smem_u32(s.tail_bar), tail_cluster = ptx::map_to_rank(tail_own, rank);
+    const uint32_t smem0 = ptx::smem_u32(s.stages);
     int stage = 0;
     uint32_t phase = 0, tail_phase = 0;
     bool ok = true;
@@ -378,25 +413,23 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       const int local = tile - g * per_group;
       const int n0 = local / p.k_blocks * kGrpTile + static_cast<int>(rank) * 128;
       const int k0 = local % p.k_blocks * kGrpTile + static_cast<int>(rank) * 128;
-      const int row0 = s.starts[g];
-      const int size = s.starts[g + 1] - row0;
+      const int row0 = ptx::uniform(s.starts[g]);
+      const int size = ptx::uniform(s.starts[g + 1]) - row0;
       for (int done = 0; done < size; done += kGrpStageK) {
-        if (!ptx::mbar_wait(ptx::smem_u32(&s.empty_bar[stage]), phase ^ 1u, s.abort_flag)) { ok = false; break; }
-        const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(&s.full_bar[stage]), 0);
+        if (!ptx::mbar_wait(empty_own + 8 * stage, phase ^ 1u, s.abort_flag)) { ok = false; break; }
         const int live = min(kGrpStageK, size - done);
         const bool ragged = (live & 15) != 0;
-        uint8_t* st = s.stages + stage * kGrpStageBytes;
-        const uint32_t sa = ptx::smem_u32(st);
-        if (lane == 0) {
-          uint32_t bar = full0;
+        if (ptx::elect_one()) {
+          uint32_t bar = full0 + 8 * stage;
+          const uint32_t sa = smem0 + stage * kGrpStageBytes;
           if (ragged) {
             // the bytes of this CTA are waited for here; rank 0's barrier then gets one arrival from each CTA
-            bar = ptx::map_to_rank(ptx::smem_u32(s.tail_bar), rank);
-            ptx::mbar_arrive_expect_tx(ptx::smem_u32(s.tail_bar), kGrpStageBytes);
+            bar = tail_cluster;
+            ptx::mbar_arrive_expect_tx(tail_own, kGrpStageBytes);
           } else if (rank == 0) {
-            ptx::mbar_arrive_expect_tx(ptx::smem_u32(&s.full_bar[stage]), 2 * kGrpStageBytes);
+            ptx::mbar_arrive_expect_tx(full_own + 8 * stage, 2 * kGrpStageBytes);
           } else {
-            ptx::mbar_arrive_cluster(full0);
+            ptx::mbar_arrive_cluster(full0 + 8 * stage);
           }
           const int r = row0 + done;
 #pragma unroll
@@ -405,11 +438,12 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
             ptx::tma_load_2d_pair(sa + kGrpOperandBytes + c * (kGrpOperandBytes / 2), &tm_x, bar, k0 + 64 * c, r);
           }
         }
+        __syncwarp();
         if (ragged) {
-          __syncwarp();
-          if (!ptx::mbar_wait(ptx::smem_u32(s.tail_bar), tail_phase, s.abort_flag)) { ok = false; break; }
+          if (!ptx::mbar_wait(tail_own, tail_phase, s.abort_flag)) { ok = false; break; }
           tail_phase ^= 1u;
           const int last = (live + 15) & ~15;
+          uint8_t* st = s.stages + stage * kGrpStageBytes;
           // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
           for (int i = lane; i < (last - live) * 32; i += 32) {
             const int row = live + (i >> 5);
@@ -418,17 +452,24 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
           }
           ptx::fence_proxy_async();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(full0);
+          if (ptx::elect_one()) ptx::mbar_arrive_cluster(full0 + 8 * stage);
+          __syncwarp();
         }
         if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
       }
     }
     if (!ok && lane == 0) grouped_fail(p, 0x11);
-    if (lane == 0) ptx::pdl_release();
+    ptx::pdl_release();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (rank 0 only)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint64_t kDesc = ptx::sw128_mnmajor_desc_template(kGrpOperandBytes / 2);
+      const uint32_t smem0 = ptx::smem_u32(s.stages);
+      const uint64_t da0 = ptx::make_smem_desc(kDesc, smem0);
+      const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kGrpOperandBytes);
+      const uint32_t full_own = ptx::smem_u32(s.full_bar), empty_own = ptx::smem_u32(s.empty_bar);
+      const uint32_t empty_peer = ptx::map_to_rank(empty_own, 1);
+      const uint32_t acc_full = ptx::smem_u32(s.acc_full_bar), acc_full_peer = ptx::map_to_rank(acc_full, 1);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -436,32 +477,36 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       bool ok = true;
       for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
         const int g = tile / per_group;
-        const int size = s.starts[g + 1] - s.starts[g];
+        const int size = ptx::uniform(s.starts[g + 1] - s.starts[g]);
         if (size == 0) continue;
         if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_empty_bar[acc]), acc_phase ^ 1u, s.abort_flag)) { ok = false; break; }
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGrpTile);
         for (int done = 0; done < size; done += kGrpStageK) {
-          if (!ptx::mbar_wait_cluster(ptx::smem_u32(&s.full_bar[stage]), phase, s.abort_flag)) { ok = false; break; }
+          if (!ptx::mbar_wait_cluster(full_own + 8 * stage, phase, s.abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
-          const uint32_t sa = ptx::smem_u32(s.stages + stage * kGrpStageBytes);
-          const uint64_t da = ptx::make_smem_desc(kDesc, sa);
-          const uint64_t db = ptx::make_smem_desc(kDesc, sa + kGrpOperandBytes);
-          const int steps = (min(kGrpStageK, size - done) + 15) >> 4;
-          for (int kk = 0; kk < steps; ++kk)
-            ptx::umma_f16_pair(d_tmem, da + kk * 128, db + kk * 128, p.idesc, (done | kk) ? 1u : 0u);
-          const uint32_t e_local = ptx::smem_u32(&s.empty_bar[stage]);
-          ptx::umma_commit_pair(e_local);
-          ptx::umma_commit_pair(ptx::map_to_rank(e_local, 1));
+          if (ptx::elect_one()) {
+            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kGrpStageBytes >> 4));
+            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kGrpStageBytes >> 4));
+            const int live = size - done;
+#pragma unroll
+            for (int kk = 0; kk < kGrpStageK / 16; ++kk)
+              if (kk * 16 < live) ptx::umma_f16_pair(d_tmem, da + kk * 128, db + kk * 128, p.idesc, (done | kk) ? 1u : 0u);
+            ptx::umma_commit_pair(empty_own + 8 * stage);
+            ptx::umma_commit_pair(empty_peer + 8 * stage);
+          }
+          __syncwarp();
           if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        const uint32_t f_local = ptx::smem_u32(&s.acc_full_bar[acc]);
-        ptx::umma_commit_pair(f_local);
-        ptx::umma_commit_pair(ptx::map_to_rank(f_local, 1));
+        if (ptx::elect_one()) {
+          ptx::umma_commit_pair(acc_full + 8 * acc);
+          ptx::umma_commit_pair(acc_full_peer + 8 * acc);
+        }
+        __syncwarp();
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok) grouped_fail(p, 0x12);
+      if (!ok && lane == 0) grouped_fail(p, 0x12);
     }
   } else {
     // ------------------------------------------------------------------ epilogue warps (both ranks)
