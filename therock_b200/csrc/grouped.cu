@@ -46,25 +46,27 @@ CUresult weight_map(CUtensorMap* tm, int dtype, const void* base, int groups, in
 }
 
 template <typename Kernel, typename... Args>
-cudaError_t launch_grouped(Kernel kernel, bool (&configured)[kMaxDevices], int pairs, cudaStream_t stream, const Args&... args) {
+cudaError_t launch_grouped(Kernel kernel, bool (&configured)[kMaxDevices], int pairs, int threads, int smem, cudaStream_t stream,
+                           const Args&... args) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGrpSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(2 * pairs), dim3(kGrpThreads), kGrpSmemBytes, stream, args...);
+  return launch_pdl(kernel, dim3(2 * pairs), dim3(threads), smem, stream, args...);
 }
 template <bool kBf16, bool kMn>
 cudaError_t launch_rows(const CUtensorMap& w, const RowMaps& x, const GroupedParams& p, int pairs, cudaStream_t stream) {
   static bool configured[kMaxDevices] = {false};
-  return launch_grouped(fmoe_grouped_rows_kernel<kBf16, kMn>, configured, pairs, stream, w, x, p);
+  return launch_grouped(fmoe_grouped_rows_kernel<kBf16, kMn>, configured, pairs, kGrpThreads, kGrpSmemBytes, stream, w, x, p);
 }
 template <bool kBf16>
-cudaError_t launch_wgrad(const CUtensorMap& dy, const CUtensorMap& x, const GroupedParams& p, int pairs, cudaStream_t stream) {
+cudaError_t launch_wgrad(const CUtensorMap& dy, const CUtensorMap& x, const CUtensorMap& dw, const GroupedParams& p, int pairs,
+                         cudaStream_t stream) {
   static bool configured[kMaxDevices] = {false};
-  return launch_grouped(fmoe_grouped_wgrad_kernel<kBf16>, configured, pairs, stream, dy, x, p);
+  return launch_grouped(fmoe_grouped_wgrad_kernel<kBf16>, configured, pairs, kWgThreads, kWgSmemBytes, stream, dy, x, dw, p);
 }
 
 int pairs_for(int64_t tiles) {
@@ -130,9 +132,10 @@ extern "C" int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const in
     FMOE_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(groups) * n * k * 2, stream));
     return FMOE_OK;
   }
-  CUtensorMap tdy, tx;
+  CUtensorMap tdy, tx, tdw;
   CUresult r = row_map(&tdy, dtype, dy, rows, n, kGrpStageK);
   if (r == CUDA_SUCCESS) r = row_map(&tx, dtype, x, rows, k, kGrpStageK);
+  if (r == CUDA_SUCCESS) r = weight_map(&tdw, dtype, dw, groups, n, k, 32);
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_grouped_matmul_wgrad: tensor map (driver code %d)", static_cast<int>(r));
   GroupedParams p{};
   p.offsets = offsets;
@@ -146,6 +149,6 @@ extern "C" int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const in
   p.status = status;
   p.idesc = ptx::make_idesc(dtype == FMOE_BF16 ? 1u : 0u, 256, 256) | ptx::kIdescAMnMajor | ptx::kIdescBMnMajor;
   const int pairs = pairs_for(static_cast<int64_t>(groups) * p.m_blocks * p.k_blocks);
-  FMOE_CUDA(dtype == FMOE_BF16 ? launch_wgrad<true>(tdy, tx, p, pairs, stream) : launch_wgrad<false>(tdy, tx, p, pairs, stream));
+  FMOE_CUDA(dtype == FMOE_BF16 ? launch_wgrad<true>(tdy, tx, tdw, p, pairs, stream) : launch_wgrad<false>(tdy, tx, tdw, p, pairs, stream));
   return FMOE_OK;
 }

@@ -32,10 +32,13 @@ constexpr int kGrpStageBytes = 2 * kGrpOperandBytes;
 constexpr int kGrpStageK = 64;                              // 16-bit elements of the contraction per stage
 constexpr int kGrpTile = 256;
 constexpr int kGrpMisc = 256 + 2 * (kGrpMaxGroups + 8) * 4; // barriers, group starts, cumulative chunks
-constexpr int kGrpStageWords = 20;                          // row pitch of a warp's transpose area, in words
-constexpr int kGrpEpiBytes = 4 * 32 * kGrpStageWords * 4;
-constexpr int kGrpSmemBytes = kGrpStages * kGrpStageBytes + kGrpMisc + kGrpEpiBytes + 1024;
-static_assert(kGrpSmemBytes <= 227 * 1024, "shared memory budget");
+constexpr int kGrpSmemBytes = kGrpStages * kGrpStageBytes + kGrpMisc + 1024;
+// wgrad: one stage less, which leaves room for two 64-column x 32-row store buffers per epilogue warp
+constexpr int kWgThreads = kGrpThreads + 32;                // and a warp for ragged last stages
+constexpr int kWgStages = 5;
+constexpr int kWgStoreBytes = 32 * 128;
+constexpr int kWgSmemBytes = kWgStages * kGrpStageBytes + 4 * 2 * kWgStoreBytes + kGrpMisc + 1024;
+static_assert(kGrpSmemBytes <= 227 * 1024 && kWgSmemBytes <= 227 * 1024, "shared memory budget");
 
 enum : int { kStatusGroupedTimeout = 0x500 };
 
@@ -126,58 +129,57 @@ __device__ __forceinline__ RowsTile decode_rows_tile(int tile, const int* starts
   return t;
 }
 
+template <int kStages, int kStoreBytes>
 struct GroupedSmem {
-  uint8_t* stages;
+  uint8_t *stages, *store;
   uint64_t *full_bar, *empty_bar, *acc_full_bar, *acc_empty_bar, *tail_bar;
   uint32_t* tmem_slot;
   volatile int* abort_flag;
   int *starts, *cum;
-  uint32_t* epi;
-};
-__device__ __forceinline__ GroupedSmem carve_grouped_smem(uint8_t* raw) {
-  GroupedSmem s;
-  s.stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* misc = s.stages + kGrpStages * kGrpStageBytes;
-  s.full_bar = reinterpret_cast<uint64_t*>(misc);       // used in rank 0
-  s.empty_bar = s.full_bar + kGrpStages;                // both ranks
-  s.acc_full_bar = s.empty_bar + kGrpStages;            // [2] both ranks
-  s.acc_empty_bar = s.acc_full_bar + 2;                 // [2] used in rank 0
-  s.tail_bar = s.acc_empty_bar + 2;                     // wgrad: ragged last stage of this CTA
-  s.tmem_slot = reinterpret_cast<uint32_t*>(s.tail_bar + 1);
-  s.abort_flag = reinterpret_cast<volatile int*>(s.tmem_slot + 1);
-  s.starts = reinterpret_cast<int*>(misc + 256);
-  s.cum = s.starts + kGrpMaxGroups + 8;
-  s.epi = reinterpret_cast<uint32_t*>(misc + kGrpMisc);
-  return s;
-}
 
-// Barriers, tensor memory, group table.  `full_count`: arrivals per stage besides the bytes.
-__device__ __forceinline__ uint32_t grouped_setup(const GroupedSmem& s, const GroupedParams& p, int full_count, int warp) {
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kGrpStages; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&s.full_bar[i]), full_count);
-      ptx::mbar_init(ptx::smem_u32(&s.empty_bar[i]), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      ptx::mbar_init(ptx::smem_u32(&s.acc_full_bar[b]), 1);
-      ptx::mbar_init(ptx::smem_u32(&s.acc_empty_bar[b]), 8);      // 4 epilogue warps in each CTA
-    }
-    ptx::mbar_init(ptx::smem_u32(s.tail_bar), 1);
-    *s.abort_flag = 0;
-    ptx::fence_barrier_init();
-    ptx::fence_proxy_async();
+  __device__ __forceinline__ explicit GroupedSmem(uint8_t* raw) {
+    stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    store = stages + kStages * kGrpStageBytes;
+    uint8_t* misc = store + kStoreBytes;
+    full_bar = reinterpret_cast<uint64_t*>(misc);       // used in rank 0
+    empty_bar = full_bar + kStages;                     // both ranks
+    acc_full_bar = empty_bar + kStages;                 // [2] both ranks
+    acc_empty_bar = acc_full_bar + 2;                   // [2] used in rank 0
+    tail_bar = acc_empty_bar + 2;                       // [kStages] wgrad: this CTA's bytes of a ragged stage
+    tmem_slot = reinterpret_cast<uint32_t*>(tail_bar + kStages);
+    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    starts = reinterpret_cast<int*>(misc + 256);
+    cum = starts + kGrpMaxGroups + 8;
   }
-  if (warp == 1) {
-    ptx::tmem_alloc_pair(ptx::smem_u32(s.tmem_slot), 512);
-    ptx::tmem_relinquish_pair();
+
+  // Barriers, tensor memory, group table.  `full_count`: arrivals per stage besides the bytes.
+  __device__ __forceinline__ uint32_t setup(const GroupedParams& p, int full_count, int warp) const {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kStages; ++i) {
+        ptx::mbar_init(ptx::smem_u32(&full_bar[i]), full_count);
+        ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 1);
+        ptx::mbar_init(ptx::smem_u32(&tail_bar[i]), 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        ptx::mbar_init(ptx::smem_u32(&acc_full_bar[b]), 1);
+        ptx::mbar_init(ptx::smem_u32(&acc_empty_bar[b]), 8);      // 4 epilogue warps in each CTA
+      }
+      *abort_flag = 0;
+      ptx::fence_barrier_init();
+      ptx::fence_proxy_async();
+    }
+    if (warp == 1) {
+      ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512);
+      ptx::tmem_relinquish_pair();
+    }
+    ptx::pdl_wait();              // the offsets and operands of this call are read from here on
+    if (warp == 2) scan_groups(p.offsets, p.groups, p.rows, kGrpTile, starts, cum);
+    ptx::tc_fence_before();
+    ptx::cluster_sync_all();      // both CTAs' barriers are initialised before anyone signals them
+    ptx::tc_fence_after();
+    return *tmem_slot;
   }
-  ptx::pdl_wait();              // the offsets and operands of this call are read from here on
-  if (warp == 2) scan_groups(p.offsets, p.groups, p.rows, kGrpTile, s.starts, s.cum);
-  ptx::tc_fence_before();
-  ptx::cluster_sync_all();      // both CTAs' barriers are initialised before anyone signals them
-  ptx::tc_fence_after();
-  return *s.tmem_slot;
-}
+};
 
 __device__ __forceinline__ void grouped_teardown(uint32_t tmem_base, int warp) {
   // neither CTA leaves while its partner can still signal its barriers or read its shared memory
@@ -200,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGrpThreads, 1)
 fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ RowMaps tm_x,
                          const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
-  const GroupedSmem s = carve_grouped_smem(smem_raw);
+  const GroupedSmem<kGrpStages, 0> s(smem_raw);
   const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
@@ -208,7 +210,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     ptx::prefetch_tensormap(&tm_w);
     for (int i = 0; i < 4; ++i) ptx::prefetch_tensormap(&tm_x.m[i]);
   }
-  const uint32_t tmem_base = grouped_setup(s, p, 1, warp);
+  const uint32_t tmem_base = s.setup(p, 1, warp);
   const int total_tiles = s.cum[p.groups] * p.m_blocks;
   const int first_tile = blockIdx.x >> 1;
   const int tile_step = gridDim.x >> 1;
@@ -378,22 +380,25 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
 // dW_g [N, K] in 256 x 256 tiles.  The contraction runs over the group's rows, 64 per stage and 16
 // per MMA, from the group's first row on (a TMA box may start at any row).  The last stage issues
 // only the MMAs it has rows for; where the last 16 are not full, the rest of them holds rows of the
-// next group (or whatever lies behind the last one, which may be infinite or NaN), so both CTAs'
-// producer warps overwrite those rows with zeros before the MMA may read them.
+// next group (or whatever lies behind the last one, which may be infinite or NaN), so a warp of
+// each CTA overwrites those rows with zeros before the MMA may read them.  With one tile per 256
+// rows of a group the result is most of the traffic: it leaves through shared memory by TMA, which
+// cuts what lies outside of [N, K].
 template <bool kBf16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGrpThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
 fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __grid_constant__ CUtensorMap tm_x,
-                          const GroupedParams p) {
+                          const __grid_constant__ CUtensorMap tm_dw, const GroupedParams p) {
   extern __shared__ uint8_t smem_raw[];
-  const GroupedSmem s = carve_grouped_smem(smem_raw);
+  const GroupedSmem<kWgStages, 4 * 2 * kWgStoreBytes> s(smem_raw);
   const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_dy);
     ptx::prefetch_tensormap(&tm_x);
+    ptx::prefetch_tensormap(&tm_dw);
   }
-  const uint32_t tmem_base = grouped_setup(s, p, 2, warp);
+  const uint32_t tmem_base = s.setup(p, 2, warp);
   const int per_group = p.m_blocks * p.k_blocks;
   const int total_tiles = p.groups * per_group;
   const int first_tile = blockIdx.x >> 1;
@@ -406,7 +411,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
     const uint32_t tail_own = ptx::smem_u32(s.tail_bar), tail_cluster = ptx::map_to_rank(tail_own, rank);
     const uint32_t smem0 = ptx::smem_u32(s.stages);
     int stage = 0;
-    uint32_t phase = 0, tail_phase = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const int g = tile / per_group;
@@ -423,9 +428,10 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
           uint32_t bar = full0 + 8 * stage;
           const uint32_t sa = smem0 + stage * kGrpStageBytes;
           if (ragged) {
-            // the bytes of this CTA are waited for here; rank 0's barrier then gets one arrival from each CTA
-            bar = tail_cluster;
-            ptx::mbar_arrive_expect_tx(tail_own, kGrpStageBytes);
+            // this CTA's bytes are waited for by its tail warp; rank 0's barrier then gets one arrival
+            // from each CTA
+            bar = tail_cluster + 8 * stage;
+            ptx::mbar_arrive_expect_tx(tail_own + 8 * stage, kGrpStageBytes);
           } else if (rank == 0) {
             ptx::mbar_arrive_expect_tx(full_own + 8 * stage, 2 * kGrpStageBytes);
           } else {
@@ -439,23 +445,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
           }
         }
         __syncwarp();
-        if (ragged) {
-          if (!ptx::mbar_wait(tail_own, tail_phase, s.abort_flag)) { ok = false; break; }
-          tail_phase ^= 1u;
-          const int last = (live + 15) & ~15;
-          uint8_t* st = s.stages + stage * kGrpStageBytes;
-          // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
-          for (int i = lane; i < (last - live) * 32; i += 32) {
-            const int row = live + (i >> 5);
-            const int c = (i >> 3) & 3;
-            *reinterpret_cast<uint4*>(st + c * (kGrpOperandBytes / 2) + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          ptx::fence_proxy_async();
-          __syncwarp();
-          if (ptx::elect_one()) ptx::mbar_arrive_cluster(full0 + 8 * stage);
-          __syncwarp();
-        }
-        if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+        if (++stage == kWgStages) { stage = 0; phase ^= 1u; }
       }
     }
     if (!ok && lane == 0) grouped_fail(p, 0x11);
@@ -496,7 +486,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
             ptx::umma_commit_pair(empty_peer + 8 * stage);
           }
           __syncwarp();
-          if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kWgStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         if (ptx::elect_one()) {
@@ -508,12 +498,48 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       }
       if (!ok && lane == 0) grouped_fail(p, 0x12);
     }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------------ ragged last stages (both ranks)
+    const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(s.full_bar), 0);
+    int stage = 0;
+    uint32_t phases = 0;            // bit i: parity of tail_bar[i]
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const int g = tile / per_group;
+      const int size = s.starts[g + 1] - s.starts[g];
+      if (size == 0) continue;
+      const int n_stages = (size + kGrpStageK - 1) / kGrpStageK;
+      const int last_stage = (stage + n_stages - 1) % kWgStages;
+      stage = (stage + n_stages) % kWgStages;
+      const int live = size - (n_stages - 1) * kGrpStageK;
+      if ((live & 15) == 0) continue;
+      if (!ptx::mbar_wait(ptx::smem_u32(&s.tail_bar[last_stage]), (phases >> last_stage) & 1u, s.abort_flag)) { ok = false; break; }
+      phases ^= 1u << last_stage;
+      const int end = (live + 15) & ~15;
+      uint8_t* st = s.stages + last_stage * kGrpStageBytes;
+      // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
+      for (int i = lane; i < (end - live) * 32; i += 32) {
+        const int row = live + (i >> 5);
+        const int c = (i >> 3) & 3;
+        *reinterpret_cast<uint4*>(st + c * (kGrpOperandBytes / 2) + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(full0 + 8 * last_stage);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) grouped_fail(p, 0x14);
   } else {
     // ------------------------------------------------------------------ epilogue warps (both ranks)
+    // Lane = row n of the tile.  64 columns at a time are rounded, written to the warp's buffer in the
+    // 128-byte swizzle (conflict-free) and stored as a box of 64 columns x 32 rows.
     const int quad = warp & 3;
-    uint32_t* stage_w = s.epi + quad * (32 * kGrpStageWords);
+    uint8_t* buf = s.store + quad * (2 * kWgStoreBytes);
+    uint8_t* row_at = buf + lane * 128;
+    const uint32_t sw = static_cast<uint32_t>(lane & 7);
     int acc = 0;
     uint32_t acc_phase = 0;
+    int b = 0;
     bool ok = true;
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const int g = tile / per_group;
@@ -526,35 +552,36 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
         ptx::tc_fence_after();
       }
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);
-      uint16_t* o = p.out + (static_cast<size_t>(g) * p.n + n0) * p.k + k0;
-      const int cols = min(kGrpTile, p.k - k0);
-      for (int c = 0; c < cols; c += 32) {
-        uint32_t v[32];
+      const int cols = n0 < p.n ? min(kGrpTile, p.k - k0) : 0;
+      for (int c = 0; c < cols; c += 64) {
+        uint32_t v[2][32];
         if (!empty) {
-          ptx::tmem_ld_32x32(t_addr + c, v);
+          ptx::tmem_ld_32x32(t_addr + c, v[0]);
+          ptx::tmem_ld_32x32(t_addr + c + 32, v[1]);
           ptx::tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0u;
+          for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = 0u;
         }
-        uint4* mine = reinterpret_cast<uint4*>(stage_w + lane * kGrpStageWords);
+        if (lane == 0) ptx::bulk_wait_read<1>();        // the store before last has left this buffer
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          mine[q] = make_uint4(pack16<kBf16>(__uint_as_float(v[8 * q]), __uint_as_float(v[8 * q + 1])),
-                               pack16<kBf16>(__uint_as_float(v[8 * q + 2]), __uint_as_float(v[8 * q + 3])),
-                               pack16<kBf16>(__uint_as_float(v[8 * q + 4]), __uint_as_float(v[8 * q + 5])),
-                               pack16<kBf16>(__uint_as_float(v[8 * q + 6]), __uint_as_float(v[8 * q + 7])));
-        __syncwarp();
-        // 4 lanes per row, 8 rows per store instruction: 64 contiguous bytes per row
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const int r = it * 8 + (lane >> 2);
-          const int seg = (lane & 3) * 8;
-          if (n0 + r < p.n && c + seg < cols)
-            *reinterpret_cast<uint4*>(o + static_cast<size_t>(r) * p.k + c + seg) =
-                *reinterpret_cast<const uint4*>(stage_w + r * kGrpStageWords + seg / 2);
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t* f = v[q >> 2] + 8 * (q & 3);
+          *reinterpret_cast<uint4*>(row_at + b * kWgStoreBytes + ((static_cast<uint32_t>(q) ^ sw) << 4)) =
+              make_uint4(pack16<kBf16>(__uint_as_float(f[0]), __uint_as_float(f[1])),
+                         pack16<kBf16>(__uint_as_float(f[2]), __uint_as_float(f[3])),
+                         pack16<kBf16>(__uint_as_float(f[4]), __uint_as_float(f[5])),
+                         pack16<kBf16>(__uint_as_float(f[6]), __uint_as_float(f[7])));
         }
+        ptx::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::tma_store_3d(&tm_dw, ptx::smem_u32(buf + b * kWgStoreBytes), k0 + c, n0, g);
+          ptx::bulk_commit();
+        }
+        __syncwarp();
+        b ^= 1;
       }
       if (empty) continue;
       ptx::tc_fence_before();
@@ -563,6 +590,8 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (!ok && threadIdx.x == 64) grouped_fail(p, 0x13);
+    if (lane == 0) ptx::bulk_wait<0>();
+    __syncwarp();
   }
   grouped_teardown(tmem_base, warp);
 }
