@@ -132,7 +132,7 @@ __device__ __forceinline__ RowsTile decode_rows_tile(int tile, const int* starts
 template <int kStages, int kStoreBytes>
 struct GroupedSmem {
   uint8_t *stages, *store;
-  uint64_t *full_bar, *empty_bar, *acc_full_bar, *acc_empty_bar, *tail_bar;
+  uint64_t *full_bar, *empty_bar, *acc_full_bar, *acc_empty_bar, *tail_bar, *peer_bar;
   uint32_t* tmem_slot;
   volatile int* abort_flag;
   int *starts, *cum;
@@ -146,19 +146,21 @@ struct GroupedSmem {
     acc_full_bar = empty_bar + kStages;                 // [2] both ranks
     acc_empty_bar = acc_full_bar + 2;                   // [2] used in rank 0
     tail_bar = acc_empty_bar + 2;                       // [kStages] wgrad: this CTA's bytes of a ragged stage
-    tmem_slot = reinterpret_cast<uint32_t*>(tail_bar + kStages);
+    peer_bar = tail_bar + kStages;                      // [kStages] used in rank 0: the peer's ragged stage is ready
+    tmem_slot = reinterpret_cast<uint32_t*>(peer_bar + kStages);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     starts = reinterpret_cast<int*>(misc + 256);
     cum = starts + kGrpMaxGroups + 8;
   }
 
-  // Barriers, tensor memory, group table.  `full_count`: arrivals per stage besides the bytes.
-  __device__ __forceinline__ uint32_t setup(const GroupedParams& p, int full_count, int warp) const {
+  // Barriers, tensor memory, group table.
+  __device__ __forceinline__ uint32_t setup(const GroupedParams& p, int warp) const {
     if (threadIdx.x == 0) {
       for (int i = 0; i < kStages; ++i) {
-        ptx::mbar_init(ptx::smem_u32(&full_bar[i]), full_count);
+        ptx::mbar_init(ptx::smem_u32(&full_bar[i]), 1);
         ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 1);
         ptx::mbar_init(ptx::smem_u32(&tail_bar[i]), 1);
+        ptx::mbar_init(ptx::smem_u32(&peer_bar[i]), 1);
       }
       for (int b = 0; b < 2; ++b) {
         ptx::mbar_init(ptx::smem_u32(&acc_full_bar[b]), 1);
@@ -210,7 +212,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     ptx::prefetch_tensormap(&tm_w);
     for (int i = 0; i < 4; ++i) ptx::prefetch_tensormap(&tm_x.m[i]);
   }
-  const uint32_t tmem_base = s.setup(p, 1, warp);
+  const uint32_t tmem_base = s.setup(p, warp);
   const int total_tiles = s.cum[p.groups] * p.m_blocks;
   const int first_tile = blockIdx.x >> 1;
   const int tile_step = gridDim.x >> 1;
@@ -359,7 +361,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (!ok && threadIdx.x == 64) grouped_fail(p, 0x03);
@@ -398,7 +400,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
     ptx::prefetch_tensormap(&tm_x);
     ptx::prefetch_tensormap(&tm_dw);
   }
-  const uint32_t tmem_base = s.setup(p, 2, warp);
+  const uint32_t tmem_base = s.setup(p, warp);
   const int per_group = p.m_blocks * p.k_blocks;
   const int total_tiles = p.groups * per_group;
   const int first_tile = blockIdx.x >> 1;
@@ -428,14 +430,11 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
           uint32_t bar = full0 + 8 * stage;
           const uint32_t sa = smem0 + stage * kGrpStageBytes;
           if (ragged) {
-            // this CTA's bytes are waited for by its tail warp; rank 0's barrier then gets one arrival
-            // from each CTA
+            // this CTA's bytes are waited for by its tail warp
             bar = tail_cluster + 8 * stage;
             ptx::mbar_arrive_expect_tx(tail_own + 8 * stage, kGrpStageBytes);
           } else if (rank == 0) {
             ptx::mbar_arrive_expect_tx(full_own + 8 * stage, 2 * kGrpStageBytes);
-          } else {
-            ptx::mbar_arrive_cluster(full0 + 8 * stage);
           }
           const int r = row0 + done;
 #pragma unroll
@@ -473,7 +472,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kGrpTile);
         for (int done = 0; done < size; done += kGrpStageK) {
-          if (!ptx::mbar_wait_cluster(full_own + 8 * stage, phase, s.abort_flag)) { ok = false; break; }
+          if (!ptx::mbar_wait(full_own + 8 * stage, phase, s.abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
             const uint64_t da = da0 + static_cast<uint32_t>(stage * (kGrpStageBytes >> 4));
@@ -500,9 +499,9 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
     }
   } else if (warp == 6) {
     // ------------------------------------------------------------------ ragged last stages (both ranks)
-    const uint32_t full0 = ptx::map_to_rank(ptx::smem_u32(s.full_bar), 0);
+    const uint32_t peer0 = ptx::map_to_rank(ptx::smem_u32(s.peer_bar), 0);
     int stage = 0;
-    uint32_t phases = 0;            // bit i: parity of tail_bar[i]
+    uint32_t phases = 0;            // bit i: parity of tail_bar[i] and peer_bar[i]
     bool ok = true;
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const int g = tile / per_group;
@@ -514,7 +513,6 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       const int live = size - (n_stages - 1) * kGrpStageK;
       if ((live & 15) == 0) continue;
       if (!ptx::mbar_wait(ptx::smem_u32(&s.tail_bar[last_stage]), (phases >> last_stage) & 1u, s.abort_flag)) { ok = false; break; }
-      phases ^= 1u << last_stage;
       const int end = (live + 15) & ~15;
       uint8_t* st = s.stages + last_stage * kGrpStageBytes;
       // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
@@ -525,8 +523,15 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       }
       ptx::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(full0 + 8 * last_stage);
+      // rank 1 tells rank 0, which completes the stage for the MMAs when both halves are ready
+      if (rank == 1) {
+        if (lane == 0) ptx::mbar_arrive_cluster(peer0 + 8 * last_stage);
+      } else {
+        if (!ptx::mbar_wait_cluster(ptx::smem_u32(&s.peer_bar[last_stage]), (phases >> last_stage) & 1u, s.abort_flag)) { ok = false; break; }
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.full_bar[last_stage]));
+      }
       __syncwarp();
+      phases ^= 1u << last_stage;
     }
     if (!ok && lane == 0) grouped_fail(p, 0x14);
   } else {
@@ -586,7 +591,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       if (empty) continue;
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (!ok && threadIdx.x == 64) grouped_fail(p, 0x13);

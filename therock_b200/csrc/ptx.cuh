@@ -266,6 +266,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                : "memory");
 }
+// The same without release: for an arrival that only says that tensor memory has been read (ordered
+// by tcgen05.wait::ld and tcgen05.fence::before_thread_sync).  A release at cluster scope waits for
+// all of the thread's earlier global stores and loads to finish, which takes most of a microsecond.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // 2-D tiled load into this CTA's shared memory whose completion bytes are credited to an
 // mbarrier that may live in the peer CTA (cluster-space address).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* tm,
