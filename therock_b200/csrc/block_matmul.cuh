@@ -77,7 +77,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   float* sc_ring = reinterpret_cast<float*>(misc + kBmmMisc);
   uint32_t* epi = reinterpret_cast<uint32_t*>(sc_ring + kBmmScaleSlots * kBmmScaleSlotFloats);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_a);
@@ -111,28 +111,35 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 
   if (warp < 4) {
     ptx::setmaxnreg_dec<kBmmThinRegs>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer
+      const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar), smem0 = ptx::smem_u32(smem);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
         const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
         for (int k = 0; k < p.kb; ++k) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-          const uint32_t full = ptx::smem_u32(&full_bar[stage]);
-          const uint32_t sa = ptx::smem_u32(smem + stage * kBmmStageBytes);
-          ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
-          ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
-          ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+          if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag)) { ok = false; break; }
+          if (ptx::elect_one()) {
+            const uint32_t full = full0 + 8 * stage, sa = smem0 + stage * kBmmStageBytes;
+            ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
+            ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
+            ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+          }
+          __syncwarp();
           if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok) bmm_fail(p.status, 0x01);
+      if (!ok && lane == 0) bmm_fail(p.status, 0x01);
       ptx::pdl_release();
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issuer
+      const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
+      const uint32_t part_full0 = ptx::smem_u32(part_full_bar), part_empty0 = ptx::smem_u32(part_empty_bar);
       constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
+      const uint64_t da0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem));
+      const uint64_t db0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem) + kBmmABytes);
       int stage = 0;
       uint32_t phase = 0;
       int buf = 0;
@@ -140,22 +147,24 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
         for (int k = 0; k < p.kb; ++k) {
-          if (!ptx::mbar_wait(ptx::smem_u32(&part_empty_bar[buf]), buf_phase ^ 1u, abort_flag) ||
-              !ptx::mbar_wait(ptx::smem_u32(&full_bar[stage]), phase, abort_flag)) { ok = false; break; }
+          if (!ptx::mbar_wait(full0 + 8 * stage, phase, abort_flag) ||
+              !ptx::mbar_wait(part_empty0 + 8 * buf, buf_phase ^ 1u, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
-          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * kBmmTileN);
-          const uint32_t sa = ptx::smem_u32(smem + stage * kBmmStageBytes);
-          const uint64_t da = ptx::make_smem_desc(kDesc, sa);
-          const uint64_t db = ptx::make_smem_desc(kDesc, sa + kBmmABytes);
+          if (ptx::elect_one()) {
+            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * kBmmTileN);
+            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
+            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
-          ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
-          ptx::umma_commit(ptx::smem_u32(&part_full_bar[buf]));
+            for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
+            ptx::umma_commit(part_full0 + 8 * buf);
+            ptx::umma_commit(empty0 + 8 * stage);
+          }
+          __syncwarp();
           if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
           if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
         }
       }
-      if (!ok) bmm_fail(p.status, 0x02);
+      if (!ok && lane == 0) bmm_fail(p.status, 0x02);
     } else if (warp == 2) {
       // ---------------------------------------------------------------- scale products
       int slot = 0;
