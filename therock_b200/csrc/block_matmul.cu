@@ -65,7 +65,7 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.n_blocks = (n + kBmmTileN - 1) / kBmmTileN;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.idesc = ptx::make_idesc(0u, kBmmTileM, kBmmTileN);
+  p.idesc = ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
   const int tiles = p.m_blocks * p.n_blocks, sms = device_sm_count();
   const int grid = tiles < sms ? tiles : sms;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

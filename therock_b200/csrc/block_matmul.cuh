@@ -3,11 +3,13 @@
 //   out[i, j] = sum_b sa[i, b] sw[j / 128, b] P_b[i, j],   P_b = sum_{k in block b} a[i, k] w[j, k]
 //
 // The scales change with every block of K, so P_b is a fresh 128 x 256 accumulator in tensor memory
-// (one pipeline stage: 128 elements of K, four MMAs) and sixteen epilogue warps add it, scaled, to
-// running sums in registers: acc += P_b * (sa * sw), packed two at a time.  Warp (quadrant q, column
-// group c) owns rows 32q + lane and columns 64c .. 64c + 63, i.e. 64 sums a thread; four warps on
-// each scheduler take turns waiting for tensor memory and multiplying.  Two accumulators let the
-// MMAs of one stage run while the previous one is drained.
+// (one pipeline stage: 128 elements of K, four MMAs) and eight epilogue warps add it, scaled, to
+// running sums in registers: acc += P_b * (sa * sw), packed two at a time.  Warp (quadrant q, half h)
+// owns row 32q + lane and columns 128h .. 128h + 127, i.e. 128 sums a thread and one weight block.
+// Two accumulators let the MMAs of one stage run while the previous one is drained.
+//
+// What bounds it is the instructions of the promotion, not the MMAs: 512 packed multiply-adds per stage
+// and SM (256 cycles) and what surrounds them.
 //
 // A separate warp loads the scales of four blocks at a time, multiplies the activations' by the two
 // weight blocks' of the tile and leaves the products in shared memory, so the epilogue warps spend one
@@ -21,8 +23,8 @@
 
 namespace fmoe {
 
-constexpr int kBmmThreads = 640;          // warps 0-3: TMA, MMA, scales, idle; warps 4-19: epilogue
-constexpr int kBmmEpiWarps = 16;
+constexpr int kBmmThreads = 384;          // warps 0-3: TMA, MMA, scales, MMA; warps 4-11: epilogue
+constexpr int kBmmEpiWarps = 8;
 constexpr int kBmmStages = 4;
 constexpr int kBmmTileM = 128, kBmmTileN = 256;
 constexpr int kBmmABytes = kBmmTileM * 128;
@@ -34,9 +36,9 @@ constexpr int kBmmEpiBytes = kBmmEpiWarps * 32 * kBmmEpiPitch * 4;
 constexpr int kBmmMisc = 256;
 constexpr int kBmmSmemBytes = kBmmStages * kBmmStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
 static_assert(kBmmSmemBytes <= 227 * 1024, "shared memory budget");
-// setmaxnreg redistributes the 640 x 96 registers of the launch: what the roles take must not exceed it.
-constexpr int kBmmThinRegs = 64, kBmmFatRegs = 104;
-static_assert(128 * kBmmThinRegs + 512 * kBmmFatRegs <= kBmmThreads * 96, "register budget");
+// setmaxnreg redistributes the 384 x 168 registers of the launch: what the roles take must not exceed it.
+constexpr int kBmmThinRegs = 56, kBmmFatRegs = 224;
+static_assert(128 * kBmmThinRegs + 256 * kBmmFatRegs <= kBmmThreads * 168, "register budget");
 
 enum : int { kStatusBmmTimeout = 0x600 };
 
@@ -68,9 +70,9 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   uint8_t* misc = smem + kBmmStages * kBmmStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(misc);
   uint64_t* empty_bar = full_bar + kBmmStages;
-  uint64_t* part_full_bar = empty_bar + kBmmStages;      // [2]
-  uint64_t* part_empty_bar = part_full_bar + 2;          // [2]
-  uint64_t* sc_full_bar = part_empty_bar + 2;            // [kBmmScaleSlots]
+  uint64_t* part_full_bar = empty_bar + kBmmStages;      // [half][2]
+  uint64_t* part_empty_bar = part_full_bar + 4;          // [half][2]
+  uint64_t* sc_full_bar = part_empty_bar + 4;            // [kBmmScaleSlots]
   uint64_t* sc_empty_bar = sc_full_bar + kBmmScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty_bar + kBmmScaleSlots);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -84,11 +86,11 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     ptx::prefetch_tensormap(&tm_w);
     for (int i = 0; i < kBmmStages; ++i) {
       ptx::mbar_init(ptx::smem_u32(&full_bar[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 2);      // both halves' MMAs
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 4; ++b) {
       ptx::mbar_init(ptx::smem_u32(&part_full_bar[b]), 1);
-      ptx::mbar_init(ptx::smem_u32(&part_empty_bar[b]), kBmmEpiWarps);
+      ptx::mbar_init(ptx::smem_u32(&part_empty_bar[b]), kBmmEpiWarps / 2);
     }
     for (int i = 0; i < kBmmScaleSlots; ++i) {
       ptx::mbar_init(ptx::smem_u32(&sc_full_bar[i]), 32);
@@ -133,36 +135,41 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       }
       if (!ok && lane == 0) bmm_fail(p.status, 0x01);
       ptx::pdl_release();
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
+    } else if (warp & 1) {
+      // ---------------------------------------------------------------- MMA issuers
+      // Warp 1 multiplies the tile's first 128 weight rows, warp 3 the other 128: each half has two
+      // accumulators and epilogue warps of its own, so a half-tile's round trip -- MMAs, commit, wake-up,
+      // drain, release -- overlaps the other half's.
+      const int half = warp >> 1;
       const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
-      const uint32_t part_full0 = ptx::smem_u32(part_full_bar), part_empty0 = ptx::smem_u32(part_empty_bar);
+      const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty0 = ptx::smem_u32(part_empty_bar) + 16 * half;
       constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
-      const uint64_t da0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem));
-      const uint64_t db0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem) + kBmmABytes);
-      int stage = 0;
+      const uint32_t smem0 = ptx::smem_u32(smem);
+      const uint64_t da0 = ptx::make_smem_desc(kDesc, smem0);
+      const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kBmmABytes + half * 128 * 128);
+      const uint32_t d_tmem = tmem_base + half * 256;
+      const int my_tiles = blockIdx.x < total_tiles ? (total_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+      const long long stages = static_cast<long long>(my_tiles) * p.kb;
       uint32_t phase = 0;
-      int buf = 0;
-      uint32_t buf_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-        for (int k = 0; k < p.kb; ++k) {
-          if (!ptx::mbar_wait(full0 + 8 * stage, phase, abort_flag) ||
-              !ptx::mbar_wait(part_empty0 + 8 * buf, buf_phase ^ 1u, abort_flag)) { ok = false; break; }
+      for (long long it = 0; ok && it < stages; it += kBmmStages) {
+#pragma unroll
+        for (int st = 0; st < kBmmStages; ++st) {
+          if (it + st >= stages) break;
+          if (!ptx::mbar_wait(full0 + 8 * st, phase, abort_flag) ||
+              !ptx::mbar_wait(part_empty0 + 8 * (st & 1), ((st >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
-            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * kBmmTileN);
-            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
-            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
+            constexpr uint32_t kStep = kBmmStageBytes >> 4;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
-            ptx::umma_commit(part_full0 + 8 * buf);
-            ptx::umma_commit(empty0 + 8 * stage);
+            for (int kk = 0; kk < 4; ++kk)
+              ptx::umma_f8(d_tmem + (st & 1) * 128, da0 + (st * kStep + kk * 2), db0 + (st * kStep + kk * 2), p.idesc, kk ? 1u : 0u);
+            ptx::umma_commit(part_full0 + 8 * (st & 1));
+            ptx::umma_commit(empty0 + 8 * st);
           }
           __syncwarp();
-          if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
-          if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
         }
+        phase ^= 1u;
       }
       if (!ok && lane == 0) bmm_fail(p.status, 0x02);
     } else if (warp == 2) {
@@ -227,59 +234,57 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     // ------------------------------------------------------------------ promotion and epilogue
     ptx::setmaxnreg_inc<kBmmFatRegs>();
     const int quad = warp & 3;
-    const int cg = (warp - 4) >> 2;                      // 64-column group
+    const int half = (warp - 4) >> 2;                    // 128-column half: one weight block
     uint32_t* mine = epi + (warp - 4) * (32 * kBmmEpiPitch);
-    int buf = 0, slot = 0;
-    uint32_t buf_phase = 0, sphase = 0;
+    const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty0 = ptx::smem_u32(part_empty_bar) + 16 * half;
+    const uint32_t sc_full0 = ptx::smem_u32(sc_full_bar), sc_empty0 = ptx::smem_u32(sc_empty_bar);
+    const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 256);
+    const float* sc_base = sc_ring + half * kBmmTileM + quad * 32 + lane;
+    const int kb = p.kb, m_blocks = p.m_blocks;
+    uint32_t it = 0, group = 0;                          // stages and scale groups so far
     bool ok = true;
     const bool vec_out = (p.n & 7) == 0;
     for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
-      uint64_t acc[32];
+      const int m0 = tile % m_blocks * kBmmTileM, n0 = tile / m_blocks * kBmmTileN;
+      float acc[128];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) acc[j] = 0ull;
-      for (int k = 0; k < p.kb; ++k) {
-        if ((k & 3) == 0 && !ptx::mbar_wait(ptx::smem_u32(&sc_full_bar[slot]), sphase, abort_flag)) { ok = false; break; }
-        const float sc = sc_ring[slot * kBmmScaleSlotFloats + (2 * (k & 3) + (cg >> 1)) * kBmmTileM + quad * 32 + lane];
-        const uint64_t sc2 = ptx::pack2(sc, sc);
-        if (!ptx::mbar_wait(ptx::smem_u32(&part_full_bar[buf]), buf_phase, abort_flag)) { ok = false; break; }
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      for (int k = 0; k < kb; ++k) {
+        if ((k & 3) == 0 && !ptx::mbar_wait(sc_full0 + 8 * (group % kBmmScaleSlots), (group / kBmmScaleSlots) & 1u, abort_flag)) { ok = false; break; }
+        const float sc = sc_base[(group % kBmmScaleSlots) * kBmmScaleSlotFloats + 2 * (k & 3) * kBmmTileM];
+        if (!ptx::mbar_wait(part_full0 + 8 * (it & 1u), (it >> 1) & 1u, abort_flag)) { ok = false; break; }
         ptx::tc_fence_after();
-        const uint32_t t = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(buf * kBmmTileN + cg * 64);
-        uint32_t v[2][16];
-        ptx::tmem_ld_32x16(t, v[0]);
+        const uint32_t t = t_base + (it & 1u) * 128;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(t + c * 32, v);
           ptx::tmem_ld_wait();
-          if (c < 3) ptx::tmem_ld_32x16(t + (c + 1) * 16, v[(c + 1) & 1]);
           if (c == 3) {
-            // everything has left this accumulator: the MMAs may overwrite it
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&part_empty_bar[buf]));
+            if (ptx::elect_one()) {
+              ptx::mbar_arrive(part_empty0 + 8 * (it & 1u));
+              if ((k & 3) == 3 || k + 1 == kb) ptx::mbar_arrive(sc_empty0 + 8 * (group % kBmmScaleSlots));
+            }
+            ++it;
+            if ((k & 3) == 3 || k + 1 == kb) ++group;
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ptx::fma2(acc[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], sc2);
-        }
-        if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
-        if ((k & 3) == 3 || k + 1 == p.kb) {
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&sc_empty_bar[slot]));
-          if (++slot == kBmmScaleSlots) { slot = 0; sphase ^= 1u; }
+          for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), sc, acc[c * 32 + j]);
         }
       }
       if (!ok) break;
       // one rounding to bf16; 16 columns at a time turn through shared memory so that two lanes write
       // 32 consecutive bytes of a row
       const int row0 = m0 + quad * 32;
-      const int col0 = n0 + cg * 64;
+      const int col0 = n0 + half * 128;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 8; ++c) {
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          float lo, hi;
-          ptx::unpack2(acc[c * 8 + j], lo, hi);
-          const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+          const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c * 16 + 2 * j], acc[c * 16 + 2 * j + 1]);
           w[j] = *reinterpret_cast<const uint32_t*>(&b);
         }
         __syncwarp();
