@@ -20,6 +20,7 @@ import torch
 
 from .api import QUANT, FmoeError, _check, lib
 
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
 _DTYPE = {torch.bfloat16: 0, torch.float16: 2}
 _E4M3 = (torch.float8_e4m3fn, torch.uint8)
 _BLOCK_QUANT = ("block128", "block128_ue8m0")
@@ -44,16 +45,21 @@ def _bound():
 _status: dict = {}
 
 
-def _status_ptr(device: torch.device) -> Optional[int]:
-    t = _status.get(device.index)
-    if t is None:
+_status_addr: dict = {}
+
+
+def _status_ptr(index: int) -> Optional[int]:
+    ptr = _status_addr.get(index)
+    if ptr is None:
         if torch.cuda.is_current_stream_capturing():
             return None
+        device = torch.device("cuda", index)
         with torch.cuda.device(device):
             t = torch.zeros(1, dtype=torch.int32, device=device)
             torch.cuda.current_stream(device).synchronize()   # the word is zero before any stream's kernel may set it
-        _status[device.index] = t
-    return t.data_ptr()
+        _status[index] = t
+        ptr = _status_addr[index] = t.data_ptr()
+    return ptr
 
 
 def operator_status(device=None) -> int:
@@ -74,33 +80,39 @@ def operator_status(device=None) -> int:
 
 def _stream_of(t: torch.Tensor, stream) -> int:
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(t.device.index)
+        return _current_raw_stream(t.get_device())
     return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
 
 
 def _empty(shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
     """A result, allocated for the stream that writes it."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=like.device)
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=like.device)
 
 
-def _dense(name: str, t, device=None, align: int = 16) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous()):
-        raise FmoeError(-1, f"{name} must be a contiguous CUDA tensor")
+def _dense(name: str, t, device: int = -1, align: int = 16) -> int:
+    """Checks a tensor and returns its device index (`device`: the index it has to be on, if given)."""
+    try:
+        index = t.get_device()
+        if index < 0 or not t.is_contiguous():
+            raise FmoeError(-1, f"{name} must be a contiguous CUDA tensor")
+    except AttributeError:
+        raise FmoeError(-1, f"{name} must be a contiguous CUDA tensor") from None
     if t.data_ptr() % align:
         raise FmoeError(-1, f"{name} must be {align}-byte aligned")
-    if device is not None and t.device != device:
-        raise FmoeError(-1, f"{name} is on {t.device}, the other tensors on {device}")
+    if device >= 0 and index != device:
+        raise FmoeError(-1, f"{name} is on cuda:{index}, the other tensors on cuda:{device}")
+    return index
 
 
 def _result(name: str, out, shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
     if out is None:
         return _empty(shape, dtype, like, stream)
-    _dense(name, out, like.device)
+    _dense(name, out, like.get_device())
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise FmoeError(-1, f"{name} must be {dtype} {tuple(shape)}")
     return out
@@ -114,23 +126,26 @@ def _for_kernel(t: torch.Tensor) -> torch.Tensor:
 
 # ----------------------------------------------------------------------------- products grouped by expert
 def _check_grouped(x, weight, offsets):
-    _dense("x", x)
-    _dense("weight", weight, x.device)
-    _dense("offsets", offsets, x.device, 4)
-    if x.dtype not in _DTYPE or weight.dtype != x.dtype:
+    index = _dense("x", x)
+    _dense("weight", weight, index)
+    _dense("offsets", offsets, index, 4)
+    if x.dtype not in _DTYPE or weight.dtype is not x.dtype:
         raise FmoeError(-1, "x and weight must both be bfloat16 or both float16")
-    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
+    xs, ws = x.shape, weight.shape
+    if len(xs) != 2 or len(ws) != 3 or ws[2] != xs[1]:
         raise FmoeError(-1, "x must be [rows, k] and weight [groups, n, k]")
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1:
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.numel() != ws[0] + 1:
         raise FmoeError(-1, "offsets must be int32 [groups + 1]")
 
 
 def _grouped(x, weight, offsets, transpose: bool, out, stream):
     groups, n, k = weight.shape
-    out = _result("out", out, (x.shape[0], k if transpose else n), x.dtype, x, stream)
-    _check(_bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
-                                        _DTYPE[x.dtype], int(transpose), out.data_ptr(), _status_ptr(x.device),
-                                        _stream_of(x, stream)))
+    rows = x.shape[0]
+    out = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream)
+    rc = _bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), rows, groups, n, k, _DTYPE[x.dtype],
+                                      transpose, out.data_ptr(), _status_ptr(x.get_device()), _stream_of(x, stream))
+    if rc:
+        _check(rc)
     return out
 
 
@@ -138,9 +153,9 @@ def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.
                          stream=None) -> torch.Tensor:
     """dx [rows, k] with dx[r] = weight[g]^T dy[r] for the rows of group g, zeros for rows of none: the
     gradient of grouped_matmul with respect to x, from dy [rows, n]."""
-    _dense("dy", dy)
-    _dense("weight", weight, dy.device)
-    _dense("offsets", offsets, dy.device, 4)
+    index = _dense("dy", dy)
+    _dense("weight", weight, index)
+    _dense("offsets", offsets, index, 4)
     if dy.dtype not in _DTYPE or weight.dtype != dy.dtype:
         raise FmoeError(-1, "dy and weight must both be bfloat16 or both float16")
     if dy.dim() != 2 or weight.dim() != 3 or weight.shape[1] != dy.shape[1]:
@@ -154,9 +169,9 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
                          stream=None) -> torch.Tensor:
     """dw [groups, n, k] with dw[g] = dy[rows of g]^T x[rows of g]; zeros for a group without rows.
     Rows of no group do not enter it, whatever they hold."""
-    _dense("dy", dy)
-    _dense("x", x, dy.device)
-    _dense("offsets", offsets, dy.device, 4)
+    index = _dense("dy", dy)
+    _dense("x", x, index)
+    _dense("offsets", offsets, index, 4)
     if x.dtype not in _DTYPE or dy.dtype != x.dtype:
         raise FmoeError(-1, "dy and x must both be bfloat16 or both float16")
     if x.dim() != 2 or dy.dim() != 2 or x.shape[0] != dy.shape[0]:
@@ -166,7 +181,7 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     groups, n, k = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
     out = _result("out", out, (groups, n, k), x.dtype, x, stream)
     _check(_bound().fmoe_grouped_matmul_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
-                                              _DTYPE[x.dtype], out.data_ptr(), _status_ptr(x.device), _stream_of(x, stream)))
+                                              _DTYPE[x.dtype], out.data_ptr(), _status_ptr(x.get_device()), _stream_of(x, stream)))
     return out
 
 
@@ -216,41 +231,42 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     of 128, m and n are any."""
     if quant not in _BLOCK_QUANT:
         raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
-    _dense("a", a)
-    _dense("w", w, a.device)
+    index = _dense("a", a)
+    _dense("w", w, index)
     if a.dtype not in _E4M3 or w.dtype not in _E4M3:
         raise FmoeError(-1, "a and w must be float8_e4m3fn (or uint8 holding it)")
-    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+    if a.dim() != 2 or w.dim() != 2:
         raise FmoeError(-1, "a must be [m, k] and w [n, k]")
-    m, k = a.shape
-    n = w.shape[0]
+    (m, k), (n, wk) = a.shape, w.shape
+    if wk != k:
+        raise FmoeError(-1, "a must be [m, k] and w [n, k]")
     if k % 128:
         raise FmoeError(-2, "k must be a multiple of 128")
     blocks = k // 128
     row_bytes = 4 * blocks if quant == "block128" else (blocks + 3) // 4 * 4
-    _dense("a_scale", a_scale, a.device, 4)
-    _dense("w_scale", w_scale, a.device, 4)
-    if a_scale.dtype not in ((torch.float32, torch.uint8) if quant == "block128" else (torch.uint8,)) or \
-            tuple(a_scale.shape) != (m, row_bytes // a_scale.element_size()):
+    _dense("a_scale", a_scale, index, 4)
+    _dense("w_scale", w_scale, index, 4)
+    if not (a_scale.dtype is torch.uint8 or (a_scale.dtype is torch.float32 and quant == "block128")) or \
+            a_scale.shape != (m, row_bytes // a_scale.element_size()):
         raise FmoeError(-1, f"a_scale must hold {row_bytes} bytes for each of the {m} rows, as quantise_rows returns them")
-    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != ((n + 127) // 128, blocks):
+    if w_scale.dtype is not torch.float32 or w_scale.shape != ((n + 127) // 128, blocks):
         raise FmoeError(-1, f"w_scale must be float32 [{(n + 127) // 128}, {blocks}]")
     out = _result("out", out, (m, n), torch.bfloat16, a, stream)
     _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
-                                         QUANT[quant], out.data_ptr(), _status_ptr(a.device), _stream_of(a, stream)))
+                                         QUANT[quant], out.data_ptr(), _status_ptr(a.get_device()), _stream_of(a, stream)))
     return out
 
 
 # ----------------------------------------------------------------------------- the gated activation
 def _check_silu(gu, row_weight):
-    _dense("gu", gu)
+    index = _dense("gu", gu)
     if gu.dtype not in _DTYPE:
         raise FmoeError(-1, "gu must be bfloat16 or float16")
     if gu.dim() != 2 or gu.shape[1] % 2:
         raise FmoeError(-1, "gu must be [rows, 2 * width]")
     if row_weight is not None:
-        _dense("row_weight", row_weight, gu.device, 4)
-        if row_weight.dtype != torch.float32 or tuple(row_weight.shape) != (gu.shape[0],):
+        _dense("row_weight", row_weight, index, 4)
+        if row_weight.dtype is not torch.float32 or row_weight.shape != gu.shape[:1]:
             raise FmoeError(-1, "row_weight must be float32 [rows]")
     return gu.shape[0], gu.shape[1] // 2
 
@@ -266,7 +282,7 @@ def _silu(gu, row_weight, out, stream):
 def silu_mul_backward(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optional[torch.Tensor] = None, stream=None):
     """Gradients of silu_mul: (dgu [rows, 2 * width], dweight float32 [rows] or None)."""
     rows, width = _check_silu(gu, row_weight)
-    _dense("dy", dy, gu.device)
+    _dense("dy", dy, gu.get_device())
     if dy.dtype != gu.dtype or tuple(dy.shape) != (rows, width):
         raise FmoeError(-1, "dy must be [rows, width] of gu's type")
     dgu = _empty((rows, 2 * width), gu.dtype, gu, stream)
