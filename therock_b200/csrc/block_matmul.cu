@@ -1,5 +1,5 @@
 // Host side of the e4m3 product with block scales: checks, tensor maps, launch.
-#include "block_matmul.cuh"
+#include "block_small.cuh"
 
 #include "host.cuh"
 #include "internal.h"
@@ -29,6 +29,52 @@ cudaError_t launch_promote(const CUtensorMap& a, const CUtensorMap& w, const Blo
   return launch_pdl(fmoe_matmul_block128_kernel<kBytes>, dim3(grid), dim3(kBmmThreads), kBmmSmemBytes, stream, a, w, p);
 }
 
+template <int kNT, bool kBytes>
+int run_small(const void* a, const void* w, BlockSmallParams p, int k, int sms, cudaStream_t stream) {
+  using Cfg = BlockSmallCfg<kNT>;
+  CUtensorMap ta, tw;
+  CUresult r = byte_map(&ta, a, p.m, k, kNT);
+  if (r == CUDA_SUCCESS) r = byte_map(&tw, w, p.n, k, 128);
+  if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
+  p.t_tiles = (p.m + kNT - 1) / kNT;
+  const int tiles = p.t_tiles * ((p.n + 127) / 128);
+  // Split K while the CTAs still fit the GPU side by side and each keeps two blocks.
+  p.split = 1;
+  while (p.split < 8 && 2 * p.split <= kNT / 2 && tiles * p.split * 2 <= sms && p.kb >= 4 * p.split) p.split *= 2;
+  // A CTA alone on its SM takes the deep pipeline, two to an SM half of it each.
+  const int room = tiles * p.split <= sms ? 220 * 1024 : 113 * 1024;
+  int stages = kBsMaxStages;
+  while (stages > 2 && Cfg::smem_bytes(stages, p.split > 1) > room) --stages;
+  const int blocks_each = (p.kb + p.split - 1) / p.split;
+  p.stages = stages < blocks_each ? stages : blocks_each;
+  p.idesc = ptx::make_idesc(0u, 128, kNT);
+  static bool configured[kMaxDevices] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  auto kernel = fmoe_matmul_block128_small_kernel<kNT, kBytes>;
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
+    FMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
+  }
+  int smem = Cfg::smem_bytes(p.stages, p.split > 1);
+  if (smem < Cfg::kMinSmem) smem = Cfg::kMinSmem;
+  FMOE_CUDA(launch_pdl_cluster(kernel, dim3(tiles * p.split), dim3(Cfg::kThreads), smem, p.split, stream, ta, tw, p));
+  return FMOE_OK;
+}
+
+template <bool kBytes>
+int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p, int k, int sms, cudaStream_t stream) {
+  switch (nt) {
+    case 16: return run_small<16, kBytes>(a, w, p, k, sms, stream);
+    case 32: return run_small<32, kBytes>(a, w, p, k, sms, stream);
+    case 64: return run_small<64, kBytes>(a, w, p, k, sms, stream);
+    default: return run_small<128, kBytes>(a, w, p, k, sms, stream);
+  }
+}
+
+// Rows per tile of the kernel for few rows, 0 for the kernel with 128 x 256 tiles.
+int small_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 256 ? 128 : 0; }
+
 }  // namespace
 }  // namespace fmoe
 
@@ -51,6 +97,19 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   DeviceGuard guard(a);
   if (guard.rc() != FMOE_OK) return guard.rc();
   NvtxRange range("fmoe_matmul_block128");
+  const int sms = device_sm_count();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (const int nt = small_rows(m)) {
+    BlockSmallParams p{};
+    p.a_scale = a_scale;
+    p.w_scale = w_scale;
+    p.m = static_cast<int>(m);
+    p.n = n;
+    p.kb = k / 128;
+    p.out = static_cast<__nv_bfloat16*>(out);
+    p.status = status;
+    return quant == FMOE_QUANT_BLOCK128 ? run_small_nt<false>(nt, a, w, p, k, sms, s) : run_small_nt<true>(nt, a, w, p, k, sms, s);
+  }
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, m, k, kBmmTileM);
   if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, kBmmTileN);
@@ -66,9 +125,8 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
   p.idesc = ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
-  const int tiles = p.m_blocks * p.n_blocks, sms = device_sm_count();
+  const int tiles = p.m_blocks * p.n_blocks;
   const int grid = tiles < sms ? tiles : sms;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   FMOE_CUDA(quant == FMOE_QUANT_BLOCK128 ? launch_promote<false>(ta, tw, p, grid, s) : launch_promote<true>(ta, tw, p, grid, s));
   return FMOE_OK;
 }
