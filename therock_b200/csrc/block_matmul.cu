@@ -42,7 +42,7 @@ int run_small(const void* a, const void* w, BlockSmallParams p, int k, int sms, 
   p.split = 1;
   while (p.split < 8 && 2 * p.split <= kNT / 2 && tiles * p.split * 2 <= sms && p.kb >= 4 * p.split) p.split *= 2;
   // A CTA alone on its SM takes the deep pipeline, two to an SM half of it each.
-  const int room = tiles * p.split <= sms ? 220 * 1024 : 113 * 1024;
+  const int room = tiles * p.split <= sms || Cfg::kTmemCols == 512 ? 220 * 1024 : 113 * 1024;
   int stages = kBsMaxStages;
   while (stages > 2 && Cfg::smem_bytes(stages, p.split > 1) > room) --stages;
   const int blocks_each = (p.kb + p.split - 1) / p.split;

@@ -29,15 +29,15 @@ template <int kNT> struct BlockSmallCfg {
   static constexpr int kGroups = kNT > 64 ? 2 : 1;            // groups of four epilogue warps
   static constexpr int kCols = kNT / kGroups;                 // accumulator columns of a thread
   static constexpr int kThreads = 128 + 128 * kGroups;
-  static constexpr int kBufs = kNT <= 32 ? 8 : 256 / kNT;     // accumulators in flight
-  static constexpr int kTmemCols = kNT * kBufs;               // 128 or 256
+  static constexpr int kBufs = kNT <= 32 ? 8 : 4;             // accumulators in flight
+  static constexpr int kTmemCols = kNT * kBufs;               // 128, 256 or 512
   // No two CTAs may wait for each other's tensor memory while they hold their own (a CTA of a cluster
   // waits for its peers): with at least this much shared memory to a CTA, those that fit an SM together
   // never ask for more than its 512 columns.
-  static constexpr int kMinSmem = (kTmemCols == 128 ? 56 : 113) * 1024;
+  static constexpr int kMinSmem = (kTmemCols == 128 ? 56 : kTmemCols == 256 ? 113 : 200) * 1024;
   static constexpr int kStageBytes = kBsWBytes + kNT * 128;
   static constexpr int kScaleBytes = kBsScaleSlots * 4 * kNT * 4;
-  static_assert(kTmemCols == 128 || kTmemCols == 256, "see kMinSmem");
+  static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "see kMinSmem");
   static constexpr int smem_bytes(int stages, bool split) {
     return stages * kStageBytes + kBsMisc + kScaleBytes + (split ? kNT * 128 * 4 : 0) + 1024;
   }
@@ -217,27 +217,28 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
           !ptx::mbar_wait(part_full0 + 8 * buf, buf_phase, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after();
       const float4* sc = reinterpret_cast<const float4*>(sc_ring + (slot * 4 + j4) * kNT + col0);
+      // the whole accumulator is read before anything is added, so it is free again at once
+      uint32_t v[Cfg::kCols];
+      if constexpr (Cfg::kCols == 16) {
+        ptx::tmem_ld_32x16(t_base + buf * kNT, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+      } else {
 #pragma unroll
-      for (int c = 0; c < Cfg::kCols; c += 16) {
-        uint32_t v[16];
-        ptx::tmem_ld_32x16(t_base + buf * kNT + c, v);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = sc[c / 4 + q];
-          acc[c + 4 * q] = fmaf(__uint_as_float(v[4 * q]), f.x, acc[c + 4 * q]);
-          acc[c + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), f.y, acc[c + 4 * q + 1]);
-          acc[c + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), f.z, acc[c + 4 * q + 2]);
-          acc[c + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), f.w, acc[c + 4 * q + 3]);
-        }
+        for (int c = 0; c < Cfg::kCols; c += 32) ptx::tmem_ld_32x32(t_base + buf * kNT + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
       }
+      ptx::tmem_ld_wait();
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        ptx::mbar_arrive(part_empty0 + 8 * buf);
-        if (j4 == 3) ptx::mbar_arrive(sc_empty0 + 8 * slot);
+      if (lane == 0) ptx::mbar_arrive(part_empty0 + 8 * buf);
+#pragma unroll
+      for (int q = 0; q < Cfg::kCols / 4; ++q) {
+        const float4 f = sc[q];
+        acc[4 * q] = fmaf(__uint_as_float(v[4 * q]), f.x, acc[4 * q]);
+        acc[4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), f.y, acc[4 * q + 1]);
+        acc[4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), f.z, acc[4 * q + 2]);
+        acc[4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), f.w, acc[4 * q + 3]);
       }
       __syncwarp();
+      if (j4 == 3 && lane == 0) ptx::mbar_arrive(sc_empty0 + 8 * slot);
       if (++buf == Cfg::kBufs) { buf = 0; buf_phase ^= 1u; }
       if (j4 == 3 && ++slot == kBsScaleSlots) { slot = 0; sphase ^= 1u; }
     }
@@ -253,13 +254,13 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     }
   } else {
     // ------------------------------------------------------------------ sum over the cluster
-    const int share = kNT / p.split;
+    const int log_share = 31 - __clz(kNT / p.split), share = 1 << log_share;
     if (warp >= 4) {
       const uint32_t red0 = ptx::smem_u32(red) + static_cast<uint32_t>((rank * share) * 128 + row) * 4u;
 #pragma unroll
       for (int j = 0; j < Cfg::kCols; ++j) {
         const int c = col0 + j;
-        const uint32_t dst = ptx::map_to_rank(red0 + static_cast<uint32_t>((c & (share - 1)) * 512), static_cast<uint32_t>(c / share));
+        const uint32_t dst = ptx::map_to_rank(red0 + static_cast<uint32_t>((c & (share - 1)) * 512), static_cast<uint32_t>(c >> log_share));
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(acc[j]) : "memory");
       }
     }

@@ -222,9 +222,9 @@ silu_mul_backward_kernel(const uint4* __restrict__ gu, const uint4* __restrict__
   dgu[at + row_vec.d] = du;
 }
 
-// With row weights a row's gradient of its weight is a sum over the whole row: kTeam threads (a
-// warp, or the whole block) own a row and add up in a fixed order, so no atomics and the same
-// result every time.
+// With row weights a row's gradient of its weight is a sum over the whole row: kTeam threads (one warp
+// or four) own a row and add up in a fixed order, so no atomics and the same result every time.  A
+// thread has the loads of two vectors in flight.
 template <typename T, int kTeam>
 __global__ void __launch_bounds__(kSiluThreads)
 silu_mul_backward_weighted_kernel(const uint4* __restrict__ gu, const float* __restrict__ row_weight,
@@ -236,30 +236,42 @@ silu_mul_backward_weighted_kernel(const uint4* __restrict__ gu, const float* __r
   __shared__ float part[kSiluThreads / 32];
   const int t = threadIdx.x % kTeam;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kTeam;
-  if (row >= rows) return;             // a whole team: the block when kTeam is its size, else whole warps
-  const float w = __ldg(row_weight + row);
-  const uint4* g = gu + row * (2 * static_cast<int64_t>(row_vec));
-  const uint4* d = dy + row * row_vec;
-  uint4* o = dgu + row * (2 * static_cast<int64_t>(row_vec));
+  const bool live = row < rows;
   float dot = 0.0f;
-  for (int i = t; i < row_vec; i += kTeam) {
-    uint4 dg, du;
-    dot += silu_grad8<T, true>(__ldcs(g + i), __ldcs(g + row_vec + i), __ldcs(d + i), w, dg, du);
-    o[i] = dg;
-    o[row_vec + i] = du;
+  if (live) {
+    const float w = __ldg(row_weight + row);
+    const uint4* g = gu + row * (2 * static_cast<int64_t>(row_vec));
+    const uint4* d = dy + row * row_vec;
+    uint4* o = dgu + row * (2 * static_cast<int64_t>(row_vec));
+    for (int i = t; i < row_vec; i += 2 * kTeam) {
+      const int i2 = i + kTeam;
+      const bool two = i2 < row_vec;
+      const uint4 g0 = __ldcs(g + i), u0 = __ldcs(g + row_vec + i), d0 = __ldcs(d + i);
+      uint4 g1, u1, d1;
+      if (two) { g1 = __ldcs(g + i2); u1 = __ldcs(g + row_vec + i2); d1 = __ldcs(d + i2); }
+      uint4 dg, du;
+      dot += silu_grad8<T, true>(g0, u0, d0, w, dg, du);
+      __stcs(o + i, dg);
+      __stcs(o + row_vec + i, du);
+      if (two) {
+        dot += silu_grad8<T, true>(g1, u1, d1, w, dg, du);
+        __stcs(o + i2, dg);
+        __stcs(o + row_vec + i2, du);
+      }
+    }
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
   if (kTeam == 32) {
-    if (t == 0) dweight[row] = dot;
+    if (live && t == 0) dweight[row] = dot;
     return;
   }
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (live && t == 0) {
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kSiluThreads / 32; ++i) sum += part[i];
+    for (int i = 0; i < kTeam / 32; ++i) sum += part[(threadIdx.x >> 5) + i];
     dweight[row] = sum;
   }
 }
@@ -332,7 +344,7 @@ int run_backward(const void* gu, const float* rw, const void* dy, int64_t rows, 
       FMOE_CUDA(launch_pdl(silu_mul_backward_weighted_kernel<T, 32>, dim3(blocks(nr, kSiluThreads / 32)), dim3(kSiluThreads), 0,
                            stream, in, rw + r0, d, o, dweight + r0, nr, rv));
     } else {
-      FMOE_CUDA(launch_pdl(silu_mul_backward_weighted_kernel<T, kSiluThreads>, dim3(blocks(nr, 1)), dim3(kSiluThreads), 0,
+      FMOE_CUDA(launch_pdl(silu_mul_backward_weighted_kernel<T, 128>, dim3(blocks(nr, kSiluThreads / 128)), dim3(kSiluThreads), 0,
                            stream, in, rw + r0, d, o, dweight + r0, nr, rv));
     }
   }
