@@ -1,4 +1,5 @@
 // Host side of the e4m3 product with block scales: checks, tensor maps, launch.
+#include "block_hw.cuh"
 #include "block_small.cuh"
 
 #include "host.cuh"
@@ -16,17 +17,19 @@ CUresult byte_map(CUtensorMap* tm, const void* base, int64_t rows, int cols, int
   return encode_tensor_map(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
 }
 
-template <bool kBytes>
-cudaError_t launch_promote(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
+template <bool kHw>
+cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
   static bool configured[kMaxDevices] = {false};
+  constexpr auto kernel = kHw ? fmoe_matmul_block128_hw_kernel : fmoe_matmul_block128_kernel;
+  constexpr int kSmem = kHw ? kHwSmemBytes : kBmmSmemBytes;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(fmoe_matmul_block128_kernel<kBytes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBmmSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
-  return launch_pdl(fmoe_matmul_block128_kernel<kBytes>, dim3(grid), dim3(kBmmThreads), kBmmSmemBytes, stream, a, w, p);
+  return launch_pdl(kernel, dim3(grid), dim3(kBmmThreads), kSmem, stream, a, w, p);
 }
 
 template <int kNT, bool kBytes>
@@ -124,9 +127,10 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.n_blocks = (n + kBmmTileN - 1) / kBmmTileN;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.idesc = ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
+  const bool hw = quant == FMOE_QUANT_BLOCK128_UE8M0;
+  p.idesc = hw ? ptx::make_idesc_block_scaled(kBmmTileM, kBmmTileN) : ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
   const int tiles = p.m_blocks * p.n_blocks;
   const int grid = tiles < sms ? tiles : sms;
-  FMOE_CUDA(quant == FMOE_QUANT_BLOCK128 ? launch_promote<false>(ta, tw, p, grid, s) : launch_promote<true>(ta, tw, p, grid, s));
+  FMOE_CUDA(hw ? launch_tiles<true>(ta, tw, p, grid, s) : launch_tiles<false>(ta, tw, p, grid, s));
   return FMOE_OK;
 }

@@ -3,7 +3,7 @@
 //   out[i, j] = sum_b sa[i, b] sw[j / 128, b] P_b[i, j],   P_b = sum_{k in block b} a[i, k] w[j, k]
 //
 // The scales change with every block of K, so P_b is a fresh 128 x 256 accumulator in tensor memory
-// (one pipeline stage: 128 elements of K, four MMAs) and eight epilogue warps add it, scaled, to
+// (one pipeline stage: 128 elements of K) and eight epilogue warps add it, scaled, to
 // running sums in registers: acc += P_b * (sa * sw), packed two at a time.  Warp (quadrant q, half h)
 // owns row 32q + lane and columns 128h .. 128h + 127, i.e. 128 sums a thread and one weight block.
 // Two accumulators let the MMAs of one stage run while the previous one is drained.
@@ -61,7 +61,46 @@ __device__ __forceinline__ float ue8m0_value(uint32_t byte) {
   return __uint_as_float(byte == 0u ? 0x00400000u : (byte == 255u ? 0x7fffffffu : byte << 23));
 }
 
-template <bool kBytes>
+// A warp's 32 rows x kCols columns (lane = row) to bf16, one rounding: 16 columns at a time turn through
+// the warp's area of shared memory so that two lanes write 32 consecutive bytes of a row.
+template <int kCols>
+__device__ __forceinline__ void store_rows_bf16(const float (&acc)[kCols], uint32_t* area, __nv_bfloat16* out, int row0, int rows,
+                                                int col0, int n) {
+  const int lane = threadIdx.x & 31;
+  const bool vec_out = (n & 7) == 0;
+#pragma unroll
+  for (int c = 0; c < kCols / 16; ++c) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c * 16 + 2 * j], acc[c * 16 + 2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    __syncwarp();
+    uint4* dst = reinterpret_cast<uint4*>(area + lane * kBmmEpiPitch);
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    __syncwarp();
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const int r = it * 16 + (lane >> 1);
+      const int col = col0 + c * 16 + (lane & 1) * 8;
+      if (row0 + r < rows && col < n) {
+        const uint4 val = *reinterpret_cast<const uint4*>(area + r * kBmmEpiPitch + (lane & 1) * 4);
+        __nv_bfloat16* o = out + static_cast<size_t>(row0 + r) * n + col;
+        if (vec_out) {
+          *reinterpret_cast<uint4*>(o) = val;
+        } else {
+          const uint32_t x[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < n) reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kBmmThreads, 1)
 fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                             const BlockMatmulParams p) {
@@ -178,8 +217,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       uint32_t sphase = 0;
       bool ok = true;
       const int nb = (p.n + 127) >> 7;
-      const int pitch = scale_pitch(p.kb);
-      const bool vec = kBytes || ((p.kb & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0);
+      const bool vec = (p.kb & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0;
       for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
         const int m0 = tile % p.m_blocks * kBmmTileM, nb0 = tile / p.m_blocks * 2;
         const float* sw0 = p.w_scale + static_cast<size_t>(nb0) * p.kb;
@@ -198,20 +236,14 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[r][j] = 0.0f;
             if (row < p.m) {
-              if (kBytes) {
-                const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(row) * pitch + k));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[r][j] = ue8m0_value((b >> (8 * j)) & 0xffu);
+              const float* src = static_cast<const float*>(p.a_scale) + static_cast<size_t>(row) * p.kb + k;
+              if (vec) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(src));
+                s[r][0] = v.x; s[r][1] = v.y; s[r][2] = v.z; s[r][3] = v.w;
               } else {
-                const float* src = static_cast<const float*>(p.a_scale) + static_cast<size_t>(row) * p.kb + k;
-                if (vec) {
-                  const float4 v = __ldg(reinterpret_cast<const float4*>(src));
-                  s[r][0] = v.x; s[r][1] = v.y; s[r][2] = v.z; s[r][3] = v.w;
-                } else {
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    if (k + j < p.kb) s[r][j] = __ldg(src + j);
-                }
+                for (int j = 0; j < 4; ++j)
+                  if (k + j < p.kb) s[r][j] = __ldg(src + j);
               }
             }
           }
@@ -243,7 +275,6 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     const int kb = p.kb, m_blocks = p.m_blocks;
     uint32_t it = 0, group = 0;                          // stages and scale groups so far
     bool ok = true;
-    const bool vec_out = (p.n & 7) == 0;
     for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
       const int m0 = tile % m_blocks * kBmmTileM, n0 = tile / m_blocks * kBmmTileN;
       float acc[128];
@@ -261,55 +292,21 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
           ptx::tmem_ld_32x32(t + c * 32, v);
           ptx::tmem_ld_wait();
           if (c == 3) {
+            // everything has left this accumulator: the MMAs may overwrite it
             ptx::tc_fence_before();
-            __syncwarp();
-            if (ptx::elect_one()) {
-              ptx::mbar_arrive(part_empty0 + 8 * (it & 1u));
-              if ((k & 3) == 3 || k + 1 == kb) ptx::mbar_arrive(sc_empty0 + 8 * (group % kBmmScaleSlots));
-            }
+            ptx::mbar_arrive_if(part_empty0 + 8 * (it & 1u), lane == 0);
             ++it;
-            if ((k & 3) == 3 || k + 1 == kb) ++group;
+            if ((k & 3) == 3 || k + 1 == kb) {
+              ptx::mbar_arrive_if(sc_empty0 + 8 * (group % kBmmScaleSlots), lane == 0);
+              ++group;
+            }
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), sc, acc[c * 32 + j]);
         }
       }
       if (!ok) break;
-      // one rounding to bf16; 16 columns at a time turn through shared memory so that two lanes write
-      // 32 consecutive bytes of a row
-      const int row0 = m0 + quad * 32;
-      const int col0 = n0 + half * 128;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c * 16 + 2 * j], acc[c * 16 + 2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        __syncwarp();
-        uint4* dst = reinterpret_cast<uint4*>(mine + lane * kBmmEpiPitch);
-        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        __syncwarp();
-#pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          const int r = it * 16 + (lane >> 1);
-          const int col = col0 + c * 16 + (lane & 1) * 8;
-          if (row0 + r < p.m && col < p.n) {
-            const uint4 val = *reinterpret_cast<const uint4*>(mine + r * kBmmEpiPitch + (lane & 1) * 4);
-            __nv_bfloat16* o = p.out + static_cast<size_t>(row0 + r) * p.n + col;
-            if (vec_out) {
-              *reinterpret_cast<uint4*>(o) = val;
-            } else {
-              const uint32_t x[4] = {val.x, val.y, val.z, val.w};
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (col + e < p.n) reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
-            }
-          }
-        }
-      }
+      store_rows_bf16<128>(acc, mine, p.out, m0 + quad * 32, p.m, n0 + half * 128, p.n);
     }
     if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x04);
   }

@@ -158,41 +158,63 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       if (++buf == Cfg::kBufs) { buf = 0; buf_phase ^= 1u; }
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x12);
-  } else if (warp == 2) {
+  } else if (warp < 4) {
     // ------------------------------------------------------------------ scale products
+    // Warps 2 and 3 take turns (slots of even and odd index).  Each requests its next slot before it
+    // hands over the present one: four slots, sixteen blocks of K, are on their way from the start, as
+    // a product of few blocks is over before a second round trip to memory.
+    constexpr int kR = (kNT + 31) / 32;
     const uint32_t sc_full0 = ptx::smem_u32(sc_full_bar), sc_empty0 = ptx::smem_u32(sc_empty_bar);
     const float* sw = p.w_scale + static_cast<size_t>(n_blk) * p.kb;
     const int pitch = scale_pitch(p.kb);
-    int slot = 0;
-    uint32_t sphase = 0;
-    bool ok = true;
-    for (int k = k0; k < k1; k += 4) {
-      float w[4], s[(kNT + 31) / 32][4];
+    const bool vec = !kBytes && (p.kb & 3) == 0 && (k0 & 3) == 0 && ((k1 - k0) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0;
+    float s[2][kR][4], w[2][4];
+    auto request = [&](int k, float (&sv)[kR][4], float (&wv)[4]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = k + j < k1 ? __ldg(sw + k + j) : 0.0f;
+      for (int j = 0; j < 4; ++j) wv[j] = k + j < k1 ? __ldg(sw + k + j) : 0.0f;
 #pragma unroll
-      for (int r = 0; r < (kNT + 31) / 32; ++r) {
+      for (int r = 0; r < kR; ++r) {
         const int t = t0 + 32 * r + lane;
         const bool live = t < p.m && 32 * r + lane < kNT;
+        if (vec) {
+          float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live && k < k1) f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k));
+          sv[r][0] = f.x; sv[r][1] = f.y; sv[r][2] = f.z; sv[r][3] = f.w;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[r][j] = 0.0f;
-          if (live && k + j < k1)
-            s[r][j] = kBytes ? ue8m0_value(__ldg(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(t) * pitch + k + j))
-                             : __ldg(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k + j);
+          for (int j = 0; j < 4; ++j) {
+            sv[r][j] = 0.0f;
+            if (live && k + j < k1)
+              sv[r][j] = kBytes ? ue8m0_value(__ldg(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(t) * pitch + k + j))
+                                : __ldg(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k + j);
+          }
         }
       }
-      if (!ptx::mbar_wait(sc_empty0 + 8 * slot, sphase ^ 1u, abort_flag)) { ok = false; break; }
+    };
+    bool ok = true;
+    int n = warp - 2;                       // index of the slot's turn
+    auto hand_over = [&](int k, float (&sv)[kR][4], float (&wv)[4]) {
+      const int slot = n % kBsScaleSlots;
+      if (!ptx::mbar_wait(sc_empty0 + 8 * slot, ((n / kBsScaleSlots) & 1u) ^ 1u, abort_flag)) { ok = false; return; }
       float* dst = sc_ring + slot * 4 * kNT;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < (kNT + 31) / 32; ++r)
-          if (32 * r + lane < kNT) dst[j * kNT + 32 * r + lane] = s[r][j] * w[j];
+        for (int r = 0; r < kR; ++r)
+          if (32 * r + lane < kNT) dst[j * kNT + 32 * r + lane] = sv[r][j] * wv[j];
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(sc_full0 + 8 * slot);
       __syncwarp();
-      if (++slot == kBsScaleSlots) { slot = 0; sphase ^= 1u; }
+      n += 2;
+    };
+    int k = k0 + 4 * (warp - 2);
+    request(k, s[0], w[0]);
+    for (; ok && k < k1; k += 16) {
+      request(k + 8, s[1], w[1]);
+      hand_over(k, s[0], w[0]);
+      if (!ok || k + 8 >= k1) break;
+      request(k + 16, s[0], w[0]);
+      hand_over(k + 8, s[1], w[1]);
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x13);
   }
@@ -254,24 +276,36 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     }
   } else {
     // ------------------------------------------------------------------ sum over the cluster
-    const int log_share = 31 - __clz(kNT / p.split), share = 1 << log_share;
+    // Rank r sums the columns c with c % split == r, so that a tile with few live rows keeps every CTA
+    // busy; the sums of four columns are in flight at a time.
+    const int log_split = 31 - __clz(p.split), share = kNT >> log_split;
     if (warp >= 4) {
       const uint32_t red0 = ptx::smem_u32(red) + static_cast<uint32_t>((rank * share) * 128 + row) * 4u;
 #pragma unroll
       for (int j = 0; j < Cfg::kCols; ++j) {
         const int c = col0 + j;
-        const uint32_t dst = ptx::map_to_rank(red0 + static_cast<uint32_t>((c & (share - 1)) * 512), static_cast<uint32_t>(c >> log_share));
+        if (t0 + c >= p.m) break;
+        const uint32_t dst = ptx::map_to_rank(red0 + static_cast<uint32_t>((c >> log_split) * 512), static_cast<uint32_t>(c & (p.split - 1)));
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(acc[j]) : "memory");
       }
     }
     ptx::cluster_sync_all();
-    if (warp >= 4 && out_col < p.n) {
-      for (int j = (warp - 4) >> 2; j < share; j += Cfg::kGroups) {
-        const int t = t0 + rank * share + j;
-        if (t >= p.m) break;
-        float sum = 0.0f;
-        for (int r = 0; r < p.split; ++r) sum += red[(r * share + j) * 128 + row];
-        p.out[static_cast<size_t>(t) * p.n + out_col] = __float2bfloat16_rn(sum);
+    if (warp >= 4) {
+      const int first = ((warp - 4) >> 2) * (share / Cfg::kGroups);
+      for (int j0 = first; j0 < first + share / Cfg::kGroups; j0 += 4) {
+        if (t0 + (j0 << log_split) + rank >= p.m) break;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < p.split; ++r) {
+          const float* src = red + (r * share + j0) * 128 + row;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += j0 + j < share ? src[j * 128] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = t0 + ((j0 + j) << log_split) + rank;
+          if (j0 + j < first + share / Cfg::kGroups && t < p.m && out_col < p.n)
+            p.out[static_cast<size_t>(t) * p.n + out_col] = __float2bfloat16_rn(sum[j]);
+        }
       }
     }
   }
