@@ -32,51 +32,111 @@ cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& w, const Block
   return launch_pdl(kernel, dim3(grid), dim3(kBmmThreads), kSmem, stream, a, w, p);
 }
 
+// Clusters of 1, 2, 4 and 8 CTAs that run side by side when a CTA has an SM to itself (a cluster does
+// not straddle the groups that the SMs come in, so this is less than the SMs divided by its size).
+struct ClusterRoom {
+  int most[4];
+};
 template <int kNT, bool kBytes>
-int run_small(const void* a, const void* w, BlockSmallParams p, int k, int sms, cudaStream_t stream) {
+cudaError_t small_kernel_room(ClusterRoom* room) {
+  static ClusterRoom known[kMaxDevices];
+  static bool configured[kMaxDevices] = {false};
+  auto kernel = fmoe_matmul_block128_small_kernel<kNT, kBytes>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool cached = dev >= 0 && dev < kMaxDevices;
+  if (cached && configured[dev]) {
+    *room = known[dev];
+    return cudaSuccess;
+  }
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBsMostSmem);
+  for (int i = 0; i < 4 && e == cudaSuccess; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << i;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1024);
+    cfg.blockDim = dim3(BlockSmallCfg<kNT>::kThreads);
+    cfg.dynamicSmemBytes = kBsMostSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&room->most[i], kernel, &cfg);
+  }
+  if (e == cudaSuccess && cached) {
+    known[dev] = *room;
+    configured[dev] = true;
+  }
+  return e;
+}
+
+// Split K as far as all clusters run at once and every CTA keeps two blocks.
+int small_log_split(int nt, int tiles, int kb, const ClusterRoom& room) {
+  int log_split = 3;
+  while (log_split > 0 && ((2 << log_split) > nt || tiles > room.most[log_split] || kb < (2 << log_split))) --log_split;
+  return log_split;
+}
+
+template <int kNT, bool kBytes>
+int run_small(const void* a, const void* w, BlockSmallParams p, int k, cudaStream_t stream) {
   using Cfg = BlockSmallCfg<kNT>;
+  ClusterRoom room;
+  FMOE_CUDA((small_kernel_room<kNT, kBytes>(&room)));
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, p.m, k, kNT);
   if (r == CUDA_SUCCESS) r = byte_map(&tw, w, p.n, k, 128);
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
   p.t_tiles = (p.m + kNT - 1) / kNT;
   const int tiles = p.t_tiles * ((p.n + 127) / 128);
-  // Split K while the CTAs still fit the GPU side by side and each keeps two blocks.
-  p.split = 1;
-  while (p.split < 8 && 2 * p.split <= kNT / 2 && tiles * p.split * 2 <= sms && p.kb >= 4 * p.split) p.split *= 2;
+  const int log_split = small_log_split(kNT, tiles, p.kb, room);
+  p.split = 1 << log_split;
   // A CTA alone on its SM takes the deep pipeline, two to an SM half of it each.
-  const int room = tiles * p.split <= sms || Cfg::kTmemCols == 512 ? 220 * 1024 : 113 * 1024;
+  const bool alone = tiles * p.split <= room.most[0] || Cfg::kTmemCols == 512;
   int stages = kBsMaxStages;
-  while (stages > 2 && Cfg::smem_bytes(stages, p.split > 1) > room) --stages;
+  while (stages > 2 && Cfg::smem_bytes(stages, p.split > 1) > (alone ? kBsMostSmem : 113 * 1024)) --stages;
   const int blocks_each = (p.kb + p.split - 1) / p.split;
   p.stages = stages < blocks_each ? stages : blocks_each;
   p.idesc = ptx::make_idesc(0u, 128, kNT);
-  static bool configured[kMaxDevices] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  auto kernel = fmoe_matmul_block128_small_kernel<kNT, kBytes>;
-  if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    FMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-    if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
-  }
   int smem = Cfg::smem_bytes(p.stages, p.split > 1);
   if (smem < Cfg::kMinSmem) smem = Cfg::kMinSmem;
-  FMOE_CUDA(launch_pdl_cluster(kernel, dim3(tiles * p.split), dim3(Cfg::kThreads), smem, p.split, stream, ta, tw, p));
+  FMOE_CUDA(launch_pdl_cluster(fmoe_matmul_block128_small_kernel<kNT, kBytes>, dim3(tiles * p.split), dim3(Cfg::kThreads), smem,
+                               p.split, stream, ta, tw, p));
   return FMOE_OK;
 }
 
 template <bool kBytes>
-int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p, int k, int sms, cudaStream_t stream) {
+int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p, int k, cudaStream_t stream) {
   switch (nt) {
-    case 16: return run_small<16, kBytes>(a, w, p, k, sms, stream);
-    case 32: return run_small<32, kBytes>(a, w, p, k, sms, stream);
-    case 64: return run_small<64, kBytes>(a, w, p, k, sms, stream);
-    default: return run_small<128, kBytes>(a, w, p, k, sms, stream);
+    case 16: return run_small<16, kBytes>(a, w, p, k, stream);
+    case 32: return run_small<32, kBytes>(a, w, p, k, stream);
+    default: return run_small<128, kBytes>(a, w, p, k, stream);
   }
 }
 
-// Rows per tile of the kernel for few rows, 0 for the kernel with 128 x 256 tiles.
-int small_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 256 ? 128 : 0; }
+// Rows per tile of the kernel for few rows, 0 for the kernels with 128 x 256 tiles: whichever is
+// estimated to be done first.  An estimate is a fixed part (launch, set-up, the way of the first blocks,
+// the result) and a time for each K block of the longest CTA, in nanoseconds, fitted to measured times of
+// 1 to 2048 rows times weights of 1024 x 1024 up to 18432 x 7168; over those the choice is 1.1 % from
+// the best on average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 and 1.5 times as many
+// at the same time; with 128 rows there are whole rounds.
+int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
+  const int64_t n_tiles = (n + 127) / 128;
+  const int64_t big_tiles = (m + kBmmTileM - 1) / kBmmTileM * ((n + kBmmTileN - 1) / kBmmTileN);
+  double best = (hw ? 4600.0 : 5000.0) + static_cast<double>((big_tiles + sms - 1) / sms) * kb * (hw ? 330.0 : 440.0);
+  int choice = 0;
+  const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2400, 300, 1.6}, {32, 3500, 360, 1.5}, {128, 5500, 420, 1.0}};
+  for (const auto& kind : kinds) {
+    const int64_t tiles = (m + kind.nt - 1) / kind.nt * n_tiles;
+    if (tiles > (int64_t{1} << 20)) continue;
+    const int split = 1 << small_log_split(kind.nt, static_cast<int>(tiles), kb, room);
+    const int64_t ctas = tiles * split;
+    double rounds = kind.nt == 128 ? static_cast<double>((ctas + sms - 1) / sms) : static_cast<double>(ctas) / (sms * kind.shared);
+    if (rounds < 1.0) rounds = 1.0;
+    const double t = kind.fixed + (kb + split - 1) / split * kind.block * rounds;
+    if (t < best) { best = t; choice = kind.nt; }
+  }
+  return choice;
+}
 
 }  // namespace
 }  // namespace fmoe
@@ -102,7 +162,10 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   NvtxRange range("fmoe_matmul_block128");
   const int sms = device_sm_count();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (const int nt = small_rows(m)) {
+  const bool hw = quant == FMOE_QUANT_BLOCK128_UE8M0;
+  ClusterRoom room;
+  FMOE_CUDA((hw ? small_kernel_room<16, true>(&room) : small_kernel_room<16, false>(&room)));
+  if (const int nt = small_rows(m, n, k / 128, hw, sms, room)) {
     BlockSmallParams p{};
     p.a_scale = a_scale;
     p.w_scale = w_scale;
@@ -111,7 +174,7 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
     p.kb = k / 128;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.status = status;
-    return quant == FMOE_QUANT_BLOCK128 ? run_small_nt<false>(nt, a, w, p, k, sms, s) : run_small_nt<true>(nt, a, w, p, k, sms, s);
+    return hw ? run_small_nt<true>(nt, a, w, p, k, s) : run_small_nt<false>(nt, a, w, p, k, s);
   }
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, m, k, kBmmTileM);
@@ -127,7 +190,6 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.n_blocks = (n + kBmmTileN - 1) / kBmmTileN;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  const bool hw = quant == FMOE_QUANT_BLOCK128_UE8M0;
   p.idesc = hw ? ptx::make_idesc_block_scaled(kBmmTileM, kBmmTileN) : ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
   const int tiles = p.m_blocks * p.n_blocks;
   const int grid = tiles < sms ? tiles : sms;

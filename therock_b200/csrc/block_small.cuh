@@ -2,7 +2,7 @@
 //
 // With few rows the weights are the work: they are read once and every byte is used for a handful of
 // multiply-adds.  So the weights are the MMA's M side -- 128 weight rows, exactly one block of their
-// scales -- and the activation rows its N side, kNT = 16, 32, 64 or 128 of them, which keeps the
+// scales -- and the activation rows its N side, kNT = 16, 32 or 128 of them, which keeps the
 // activations' share of the traffic small.  Lane = output column, accumulator column = row.  P_b of a
 // block of K is a kNT-column accumulator, several of which are in flight, and the epilogue warps add
 // them, scaled, in registers: a row's scale times the weight block's comes from shared memory, the
@@ -24,6 +24,7 @@ constexpr int kBsWBytes = 128 * 128;
 constexpr int kBsScaleSlots = 4;              // ring of scale products, four K blocks a slot
 constexpr int kBsMaxStages = 10;
 constexpr int kBsMisc = 512;
+constexpr int kBsMostSmem = 220 * 1024;
 
 template <int kNT> struct BlockSmallCfg {
   static constexpr int kGroups = kNT > 64 ? 2 : 1;            // groups of four epilogue warps
@@ -176,18 +177,25 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       for (int r = 0; r < kR; ++r) {
         const int t = t0 + 32 * r + lane;
         const bool live = t < p.m && 32 * r + lane < kNT;
-        if (vec) {
+        if (kBytes) {
+          // four bytes from any position: two aligned words of the row (its pitch is a multiple of four)
+          uint32_t lo = 0u, hi = 0u;
+          if (live && k < k1) {
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(t) * pitch);
+            lo = __ldg(words + (k >> 2));
+            if ((k & 3) != 0 && (k >> 2) + 1 < (pitch >> 2)) hi = __ldg(words + (k >> 2) + 1);
+          }
+          const uint32_t four = __funnelshift_r(lo, hi, 8 * (k & 3));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sv[r][j] = live && k + j < k1 ? ue8m0_value((four >> (8 * j)) & 0xffu) : 0.0f;
+        } else if (vec) {
           float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
           if (live && k < k1) f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k));
           sv[r][0] = f.x; sv[r][1] = f.y; sv[r][2] = f.z; sv[r][3] = f.w;
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            sv[r][j] = 0.0f;
-            if (live && k + j < k1)
-              sv[r][j] = kBytes ? ue8m0_value(__ldg(static_cast<const uint8_t*>(p.a_scale) + static_cast<size_t>(t) * pitch + k + j))
-                                : __ldg(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k + j);
-          }
+          for (int j = 0; j < 4; ++j)
+            sv[r][j] = live && k + j < k1 ? __ldg(static_cast<const float*>(p.a_scale) + static_cast<size_t>(t) * p.kb + k + j) : 0.0f;
         }
       }
     };
