@@ -400,7 +400,11 @@ FMOE_API int fmoe_ep_wait_combine(const int32_t* topk_ids, int32_t T, int32_t K,
  * workspace, no device memory of their own, no host synchronisation; the same inputs give the same
  * bits (no atomics).  Matrices are row-major and dense, 16-byte aligned.  `status` (optional) is a
  * device int32 that receives a code if a bounded wait in a kernel runs out (the results are then
- * not valid); it is not cleared.  No counterpart in the reference operator. */
+ * not valid); it is not cleared.  Without it the code goes to a word of the library's, one per
+ * device, which fmoe_operator_status waits for, returns and clears.  No counterpart in the
+ * reference operator. */
+FMOE_API int fmoe_operator_status(int32_t device, int32_t* status_out);
+
 
 /* Products grouped by expert, ragged in the rows: group g owns the rows offsets[g] .. offsets[g+1]-1
  * of the row matrices (offsets: device int32[groups + 1], read as a running maximum clamped to

@@ -1,4 +1,4 @@
-"""Builds libfmoe_b200.so (sm_100a only) in-tree with nvcc."""
+"""Builds libfmoe_b200.so (sm_100a only) in-tree with nvcc, and the torch binding with g++."""
 from __future__ import annotations
 
 import os
@@ -38,7 +38,37 @@ def build(force: bool = False, verbose: bool = False, checked: bool = False, tim
     if checked or timing_switches:
         return _build_variant("checked" if checked else "timing",
                               ["-DFMOE_BOUNDS_CHECKS"] if checked else ["-DFMOE_TIMING_SWITCHES"], force, verbose)
-    return _build_variant("", [], force, verbose)
+    lib = _build_variant("", [], force, verbose)
+    build_binding(force, verbose)
+    return lib
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Builds _fmoe_torch.so, the CPython binding of the operators in ops.py (host code only, g++ and
+    torch's headers).  It does not link the library: ops.py passes it the entry points."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    out = os.path.join(HERE, "_fmoe_torch.so")
+    if not force and not _stale(out, [src, os.path.join(HERE, "..", "include", "fused_moe_c.h")]):
+        return out
+    cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{i}" for i in include], src, "-o", out,
+           f"-L{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{torch_lib}"]
+    env = {k: v for k, v in os.environ.items() if k not in ("CC", "CXX")}
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
+    if verbose or r.returncode != 0:
+        print(" ".join(cmd))
+        print(r.stdout)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for torch_binding.cpp")
+    return out
 
 
 def _build_variant(suffix: str, defines: list, force: bool, verbose: bool) -> str:

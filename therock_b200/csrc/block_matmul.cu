@@ -139,6 +139,13 @@ int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& ro
 }
 
 }  // namespace
+
+cudaError_t take_block_matmul_status(int32_t* code) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_bmm_status, sizeof(*code));
+  const int32_t zero = 0;
+  if (e == cudaSuccess && *code != 0) e = cudaMemcpyToSymbol(g_bmm_status, &zero, sizeof(zero));
+  return e;
+}
 }  // namespace fmoe
 
 extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
@@ -194,5 +201,22 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   const int tiles = p.m_blocks * p.n_blocks;
   const int grid = tiles < sms ? tiles : sms;
   FMOE_CUDA(hw ? launch_tiles<true>(ta, tw, p, grid, s) : launch_tiles<false>(ta, tw, p, grid, s));
+  return FMOE_OK;
+}
+
+extern "C" int fmoe_operator_status(int32_t device, int32_t* status_out) {
+  using namespace fmoe;
+  if (!status_out) return fail(FMOE_ERR_INVALID_ARG, "fmoe_operator_status: status_out is required");
+  *status_out = 0;
+  int before = 0;
+  FMOE_CUDA(cudaGetDevice(&before));
+  FMOE_CUDA(cudaSetDevice(device));
+  int32_t code[2] = {0, 0};
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = take_grouped_status(&code[0]);
+  if (e == cudaSuccess) e = take_block_matmul_status(&code[1]);
+  cudaSetDevice(before);
+  if (e != cudaSuccess) return fail(FMOE_ERR_CUDA, "fmoe_operator_status failed: %s", cudaGetErrorString(e));
+  *status_out = code[0] ? code[0] : code[1];
   return FMOE_OK;
 }

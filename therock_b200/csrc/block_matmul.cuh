@@ -52,8 +52,10 @@ struct BlockMatmulParams {
   uint32_t idesc;
 };
 
+static __device__ int g_bmm_status;      // for calls without a status word
+
 __device__ __forceinline__ void bmm_fail(int* status, int code) {
-  if (status != nullptr) atomicExch(status, kStatusBmmTimeout | code);
+  atomicExch(status != nullptr ? status : &g_bmm_status, kStatusBmmTimeout | code);
 }
 
 // Exponent byte -> power of two (0 is 2^-127, 255 is NaN).

@@ -75,6 +75,13 @@ int pairs_for(int64_t tiles) {
 }
 
 }  // namespace
+
+cudaError_t take_grouped_status(int32_t* code) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, g_grouped_status, sizeof(*code));
+  const int32_t zero = 0;
+  if (e == cudaSuccess && *code != 0) e = cudaMemcpyToSymbol(g_grouped_status, &zero, sizeof(zero));
+  return e;
+}
 }  // namespace fmoe
 
 extern "C" int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* offsets, int64_t rows, int32_t groups,

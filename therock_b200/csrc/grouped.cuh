@@ -65,8 +65,10 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+static __device__ int g_grouped_status;      // for calls without a status word
+
 __device__ __forceinline__ void grouped_fail(const GroupedParams& p, int code) {
-  if (p.status != nullptr) atomicExch(p.status, kStatusGroupedTimeout | code);
+  atomicExch(p.status != nullptr ? p.status : &g_grouped_status, kStatusGroupedTimeout | code);
 }
 
 // One warp: starts[0 .. G] = running maximum of the offsets clamped to [0, rows];

@@ -137,6 +137,12 @@ struct GemmLaunch {
 // tensor-map encode fails.
 cudaError_t launch_grouped_gemm(const GemmLaunch& g, cudaStream_t stream, int* drv_err);
 
+// Status words of the operators that take no workspace: a code that a kernel leaves when a bounded wait
+// runs out and the caller gave no word of its own.  One per translation unit and device, part of the
+// loaded module; take_* reads and clears the current device's.
+cudaError_t take_grouped_status(int32_t* code);
+cudaError_t take_block_matmul_status(int32_t* code);
+
 // Tensor map of a row-major array (dims and box innermost first, strides of the outer dimensions in
 // bytes, rank 2 or 3) read in 128-byte-swizzled boxes; what lies outside is filled with zeros.
 CUresult encode_tensor_map(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,

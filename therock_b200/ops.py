@@ -31,6 +31,7 @@ def _bound():
     l = lib()
     if l.fmoe_grouped_matmul.argtypes is None:
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+        l.fmoe_operator_status.argtypes = [i32, ctypes.POINTER(i32)]
         l.fmoe_grouped_matmul_wgrad.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, vp]
         l.fmoe_matmul_block128.argtypes = [vp, vp, vp, vp, i64, i32, i32, i32, vp, vp, vp]
         l.fmoe_silu_mul.argtypes = [vp, vp, i64, i32, i32, vp, vp]
@@ -40,42 +41,34 @@ def _bound():
     return l
 
 
-# One status word per device, made at the first call outside a stream capture (a tensor allocated
-# inside one would belong to that graph).  Kernels only write to it when a bounded wait runs out.
-_status: dict = {}
+_binding = None
 
 
-_status_addr: dict = {}
-
-
-def _status_ptr(index: int) -> Optional[int]:
-    ptr = _status_addr.get(index)
-    if ptr is None:
-        if torch.cuda.is_current_stream_capturing():
-            return None
-        device = torch.device("cuda", index)
-        with torch.cuda.device(device):
-            t = torch.zeros(1, dtype=torch.int32, device=device)
-            torch.cuda.current_stream(device).synchronize()   # the word is zero before any stream's kernel may set it
-        _status[index] = t
-        ptr = _status_addr[index] = t.data_ptr()
-    return ptr
+def _native():
+    """The CPython binding of the calls without `out` and `stream` (torch_binding.cpp), which also holds
+    the autograd nodes; bound to the library that api.lib() loads."""
+    global _binding
+    if _binding is None:
+        l = _bound()
+        try:
+            from . import _fmoe_torch as binding
+        except ImportError as e:
+            raise FmoeError(-100, f"the torch binding is missing or does not load ({e}): build it with "
+                                  "`python -m therock_b200.build`") from None
+        binding.bind(FmoeError, *(ctypes.cast(getattr(l, n), ctypes.c_void_p).value for n in (
+            "fmoe_grouped_matmul", "fmoe_grouped_matmul_wgrad", "fmoe_matmul_block128", "fmoe_silu_mul",
+            "fmoe_silu_mul_quantise", "fmoe_silu_mul_backward", "fmoe_last_error")))
+        _binding = binding
+    return _binding
 
 
 def operator_status(device=None) -> int:
     """Waits for the device and returns the code of the last bounded wait that ran out in one of this
     module's kernels (0: none did), and clears it."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    t = _status.get(device.index)
-    if t is None:
-        return 0
-    torch.cuda.synchronize(device)
-    code = int(t.item())
-    if code:
-        t.zero_()
-    return code
+    index = torch.device("cuda" if device is None else device).index
+    code = ctypes.c_int32(0)
+    _check(_bound().fmoe_operator_status(torch.cuda.current_device() if index is None else index, ctypes.byref(code)))
+    return int(code.value)
 
 
 def _stream_of(t: torch.Tensor, stream) -> int:
@@ -124,6 +117,11 @@ def _for_kernel(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() & 15 else t
 
 
+def _refuse_gradients(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
+
+
 # ----------------------------------------------------------------------------- products grouped by expert
 def _check_grouped(x, weight, offsets):
     index = _dense("x", x)
@@ -143,7 +141,7 @@ def _grouped(x, weight, offsets, transpose: bool, out, stream):
     rows = x.shape[0]
     out = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream)
     rc = _bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), rows, groups, n, k, _DTYPE[x.dtype],
-                                      transpose, out.data_ptr(), _status_ptr(x.get_device()), _stream_of(x, stream))
+                                      transpose, out.data_ptr(), None, _stream_of(x, stream))
     if rc:
         _check(rc)
     return out
@@ -181,24 +179,8 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     groups, n, k = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
     out = _result("out", out, (groups, n, k), x.dtype, x, stream)
     _check(_bound().fmoe_grouped_matmul_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
-                                              _DTYPE[x.dtype], out.data_ptr(), _status_ptr(x.get_device()), _stream_of(x, stream)))
+                                              _DTYPE[x.dtype], out.data_ptr(), None, _stream_of(x, stream)))
     return out
-
-
-class _GroupedMatmul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, offsets):
-        ctx.save_for_backward(x, weight, offsets)
-        return _grouped(x, weight, offsets, False, None, None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, offsets = ctx.saved_tensors
-        dy = _for_kernel(dy)
-        dx = grouped_matmul_dgrad(dy, weight, offsets) if ctx.needs_input_grad[0] else None
-        dw = grouped_matmul_wgrad(dy, x, offsets) if ctx.needs_input_grad[1] else None
-        return dx, dw, None
 
 
 def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -211,11 +193,12 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     from offsets[-1] on) give zero rows and zero gradients.  Offsets are read as a running maximum
     clamped to [0, rows].  n and k are multiples of 8, at most 1024 groups.  Differentiable in x and
     weight; `out` and `stream` are for calls without gradients."""
+    if out is None and stream is None:
+        y = (_binding or _native()).grouped_matmul(x, weight, offsets)
+        if y is not None:
+            return y
     _check_grouped(x, weight, offsets)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        if out is not None or stream is not None:
-            raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
-        return _GroupedMatmul.apply(x, weight, offsets)
+    _refuse_gradients(x, weight)
     return _grouped(x, weight, offsets, False, out, stream)
 
 
@@ -231,6 +214,10 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     of 128, m and n are any."""
     if quant not in _BLOCK_QUANT:
         raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
+    if out is None and stream is None:
+        y = (_binding or _native()).matmul_block128(a, a_scale, w, w_scale, QUANT[quant])
+        if y is not None:
+            return y
     index = _dense("a", a)
     _dense("w", w, index)
     if a.dtype not in _E4M3 or w.dtype not in _E4M3:
@@ -253,7 +240,7 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
         raise FmoeError(-1, f"w_scale must be float32 [{(n + 127) // 128}, {blocks}]")
     out = _result("out", out, (m, n), torch.bfloat16, a, stream)
     _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
-                                         QUANT[quant], out.data_ptr(), _status_ptr(a.get_device()), _stream_of(a, stream)))
+                                         QUANT[quant], out.data_ptr(), None, _stream_of(a, stream)))
     return out
 
 
@@ -293,30 +280,18 @@ def silu_mul_backward(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optional[t
     return dgu, dweight
 
 
-class _SiluMul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gu, row_weight):
-        ctx.save_for_backward(gu, row_weight)
-        return _silu(gu, row_weight, None, None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        gu, row_weight = ctx.saved_tensors
-        return silu_mul_backward(gu, _for_kernel(dy), row_weight)
-
-
 def silu_mul(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
              stream=None) -> torch.Tensor:
     """out[r, i] = row_weight[r] * SiLU(gu[r, i]) * gu[r, width + i] for gu [rows, 2 * width] in
     bfloat16 or float16 (gate columns, then up columns), row_weight float32 [rows] or none.  32-bit
     arithmetic, one rounding; width is a multiple of 8.  Differentiable in gu and row_weight; `out`
     and `stream` are for calls without gradients."""
+    if out is None and stream is None:
+        y = (_binding or _native()).silu_mul(gu, row_weight)
+        if y is not None:
+            return y
     _check_silu(gu, row_weight)
-    if torch.is_grad_enabled() and (gu.requires_grad or (row_weight is not None and row_weight.requires_grad)):
-        if out is not None or stream is not None:
-            raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
-        return _SiluMul.apply(gu, row_weight)
+    _refuse_gradients(gu, row_weight)
     return _silu(gu, row_weight, out, stream)
 
 
@@ -326,6 +301,10 @@ def silu_mul_quantise(gu: torch.Tensor, quant: str, row_weight: Optional[torch.T
     (q uint8 [rows, width], scales uint8 [rows, bytes]).  width is a multiple of 128.  No gradient."""
     if quant not in _BLOCK_QUANT:
         raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
+    if q is None and scales is None and stream is None:
+        both = (_binding or _native()).silu_mul_quantise(gu, QUANT[quant], row_weight)
+        if both is not None:
+            return both
     rows, width = _check_silu(gu, row_weight)
     if width % 128:
         raise FmoeError(-2, "width must be a multiple of 128")
