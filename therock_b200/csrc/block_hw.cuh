@@ -17,21 +17,27 @@
 
 namespace fmoe {
 
+constexpr int kHwThreads = 384;                   // warps 0-3: TMA, MMA, scale images, idle; warps 4-11: epilogue
+constexpr int kHwEpiWarps = 8;
+constexpr int kHwTileN = 256;
+constexpr int kHwStages = 4;
+constexpr int kHwStageBytes = kBmmABytes + kHwTileN * 128;
+constexpr int kHwEpiBytes = kHwEpiWarps * 32 * kBmmEpiPitch * 4;
 constexpr int kHwSfSlots = 4;                     // ring of scale images, four K blocks a slot
 constexpr int kHwSfSlotBytes = 512 + 2 * 512;     // activation rows, two weight blocks
-constexpr int kHwSfCol = kBmmTileN;               // scale columns behind the accumulator, two buffers of 16
-constexpr int kHwSmemBytes = kBmmStages * kBmmStageBytes + kBmmMisc + kHwSfSlots * kHwSfSlotBytes + kBmmEpiBytes + 1024;
+constexpr int kHwSfCol = kHwTileN;               // scale columns behind the accumulator, two buffers of 16
+constexpr int kHwSmemBytes = kHwStages * kHwStageBytes + kBmmMisc + kHwSfSlots * kHwSfSlotBytes + kHwEpiBytes + 1024;
 static_assert(kHwSmemBytes <= 227 * 1024, "shared memory budget");
 
-__global__ void __launch_bounds__(kBmmThreads, 1)
+__global__ void __launch_bounds__(kHwThreads, 1)
 fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                                const BlockMatmulParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* misc = smem + kBmmStages * kBmmStageBytes;
+  uint8_t* misc = smem + kHwStages * kHwStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(misc);
-  uint64_t* empty_bar = full_bar + kBmmStages;
-  uint64_t* sf_full_bar = empty_bar + kBmmStages;        // [kHwSfSlots]
+  uint64_t* empty_bar = full_bar + kHwStages;
+  uint64_t* sf_full_bar = empty_bar + kHwStages;        // [kHwSfSlots]
   uint64_t* sf_empty_bar = sf_full_bar + kHwSfSlots;
   uint64_t* acc_full_bar = sf_empty_bar + kHwSfSlots;
   uint64_t* acc_empty_bar = acc_full_bar + 1;
@@ -45,7 +51,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_a);
     ptx::prefetch_tensormap(&tm_w);
-    for (int i = 0; i < kBmmStages; ++i) {
+    for (int i = 0; i < kHwStages; ++i) {
       ptx::mbar_init(ptx::smem_u32(&full_bar[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&empty_bar[i]), 1);
     }
@@ -54,7 +60,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
       ptx::mbar_init(ptx::smem_u32(&sf_empty_bar[i]), 1);
     }
     ptx::mbar_init(ptx::smem_u32(acc_full_bar), 1);
-    ptx::mbar_init(ptx::smem_u32(acc_empty_bar), kBmmEpiWarps);
+    ptx::mbar_init(ptx::smem_u32(acc_empty_bar), kHwEpiWarps);
     *abort_flag = 0;
     ptx::fence_barrier_init();
     ptx::fence_proxy_async();
@@ -78,24 +84,24 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
+      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kHwTileN;
       for (int k = 0; k < p.kb; ++k) {
         if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag)) { ok = false; break; }
         if (ptx::elect_one()) {
-          const uint32_t full = full0 + 8 * stage, sa = smem0 + stage * kBmmStageBytes;
-          ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
+          const uint32_t full = full0 + 8 * stage, sa = smem0 + stage * kHwStageBytes;
+          ptx::mbar_arrive_expect_tx(full, kHwStageBytes);
           ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
           ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
         }
         __syncwarp();
-        if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
+        if (++stage == kHwStages) { stage = 0; phase ^= 1u; }
       }
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x21);
     ptx::pdl_release();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer: four K blocks at a time
-    static_assert(kBmmStages == 4, "a group of four K blocks goes once round the stages");
+    static_assert(kHwStages == 4, "a group of four K blocks goes once round the stages");
     const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t sf_full0 = ptx::smem_u32(sf_full_bar), sf_empty0 = ptx::smem_u32(sf_empty_bar), sf0 = ptx::smem_u32(sf_ring);
     const uint32_t acc_full = ptx::smem_u32(acc_full_bar), acc_empty = ptx::smem_u32(acc_empty_bar);
@@ -129,8 +135,8 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
           if (!ptx::mbar_wait(full0 + 8 * stage, phase, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
-            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
-            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kBmmStageBytes >> 4));
+            const uint64_t da = da0 + static_cast<uint32_t>(stage * (kHwStageBytes >> 4));
+            const uint64_t db = db0 + static_cast<uint32_t>(stage * (kHwStageBytes >> 4));
             const uint32_t idesc = ptx::idesc_with_scale_byte(p.idesc, u);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
@@ -138,7 +144,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
             ptx::umma_commit(empty0 + 8 * stage);
           }
           __syncwarp();
-          if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kHwStages) { stage = 0; phase ^= 1u; }
         }
       }
       if (!ok) break;
@@ -193,7 +199,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
-      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
+      const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kHwTileN;
       if (!ptx::mbar_wait(acc_full, phase, abort_flag)) { ok = false; break; }
       phase ^= 1u;
       ptx::tc_fence_after();

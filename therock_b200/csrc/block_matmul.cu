@@ -21,7 +21,7 @@ template <bool kHw>
 cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
   static bool configured[kMaxDevices] = {false};
   constexpr auto kernel = kHw ? fmoe_matmul_block128_hw_kernel : fmoe_matmul_block128_kernel;
-  constexpr int kSmem = kHw ? kHwSmemBytes : kBmmSmemBytes;
+  constexpr int kSmem = kHw ? kHwSmemBytes : kBmmSmemBytes, kThreads = kHw ? kHwThreads : kBmmThreads;
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
@@ -29,7 +29,7 @@ cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& w, const Block
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(grid), dim3(kBmmThreads), kSmem, stream, a, w, p);
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmem, stream, a, w, p);
 }
 
 // Clusters of 1, 2, 4 and 8 CTAs that run side by side when a CTA has an SM to itself (a cluster does
@@ -121,7 +121,8 @@ int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p
 // at the same time; with 128 rows there are whole rounds.
 int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
   const int64_t n_tiles = (n + 127) / 128;
-  const int64_t big_tiles = (m + kBmmTileM - 1) / kBmmTileM * ((n + kBmmTileN - 1) / kBmmTileN);
+  const int tile_n = hw ? kHwTileN : kBmmTileN;
+  const int64_t big_tiles = (m + kBmmTileM - 1) / kBmmTileM * ((n + tile_n - 1) / tile_n);
   double best = (hw ? 4600.0 : 5000.0) + static_cast<double>((big_tiles + sms - 1) / sms) * kb * (hw ? 330.0 : 440.0);
   int choice = 0;
   const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2400, 300, 1.6}, {32, 3500, 360, 1.5}, {128, 5500, 420, 1.0}};
@@ -185,7 +186,8 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   }
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, m, k, kBmmTileM);
-  if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, kBmmTileN);
+  const int tile_n = hw ? kHwTileN : kBmmTileN;
+  if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, tile_n);
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
   BlockMatmulParams p{};
   p.a_scale = a_scale;
@@ -194,10 +196,10 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.n = n;
   p.kb = k / 128;
   p.m_blocks = (p.m + kBmmTileM - 1) / kBmmTileM;
-  p.n_blocks = (n + kBmmTileN - 1) / kBmmTileN;
+  p.n_blocks = (n + tile_n - 1) / tile_n;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.idesc = hw ? ptx::make_idesc_block_scaled(kBmmTileM, kBmmTileN) : ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
+  p.idesc = hw ? ptx::make_idesc_block_scaled(kBmmTileM, kHwTileN) : ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
   const int tiles = p.m_blocks * p.n_blocks;
   const int grid = tiles < sms ? tiles : sms;
   FMOE_CUDA(hw ? launch_tiles<true>(ta, tw, p, grid, s) : launch_tiles<false>(ta, tw, p, grid, s));

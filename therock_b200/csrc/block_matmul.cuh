@@ -2,18 +2,20 @@
 // block on the weights:
 //   out[i, j] = sum_b sa[i, b] sw[j / 128, b] P_b[i, j],   P_b = sum_{k in block b} a[i, k] w[j, k]
 //
-// The scales change with every block of K, so P_b is a fresh 128 x 256 accumulator in tensor memory
-// (one pipeline stage: 128 elements of K) and eight epilogue warps add it, scaled, to
-// running sums in registers: acc += P_b * (sa * sw), packed two at a time.  Warp (quadrant q, half h)
-// owns row 32q + lane and columns 128h .. 128h + 127, i.e. 128 sums a thread and one weight block.
-// Two accumulators let the MMAs of one stage run while the previous one is drained.
+// The scales change with every block of K, so P_b is a fresh accumulator in tensor memory (one pipeline
+// stage: 128 elements of K) and eight epilogue warps add it, scaled, to running sums in registers:
+// acc += P_b * (sa * sw).  Warp (quadrant q, half h) owns row 32q + lane and columns 128h .. 128h + 127,
+// one weight block.
 //
-// What bounds it is the instructions of the promotion, not the MMAs: 512 packed multiply-adds per stage
-// and SM (256 cycles) and what surrounds them.
+// What bounds it is instructions and their latencies, not the MMAs (512 cycles a stage): issuing a
+// stage's MMAs and commits behind two waits takes a warp 600 to 800 cycles next to busy neighbours, and
+// every instruction that an epilogue warp spends besides its multiply-adds counts twice on each
+// scheduler.  So four warps issue, one to each of four 128-column accumulators (half of the tile, parity
+// of the stage), and the epilogue's loop takes four K blocks at a time with all addresses and parities in
+// registers.
 //
-// A separate warp loads the scales of four blocks at a time, multiplies the activations' by the two
-// weight blocks' of the tile and leaves the products in shared memory, so the epilogue warps spend one
-// load on them.
+// A separate warp loads the scales of four blocks at a time, multiplies the activations' by those of the
+// tile's two weight blocks and leaves the products in shared memory.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -23,7 +25,7 @@
 
 namespace fmoe {
 
-constexpr int kBmmThreads = 384;          // warps 0-3: TMA, MMA, scales, MMA; warps 4-11: epilogue
+constexpr int kBmmThreads = 512;          // warps 0, 1: TMA, scales; 4-7: MMA; 8-15: epilogue
 constexpr int kBmmEpiWarps = 8;
 constexpr int kBmmStages = 4;
 constexpr int kBmmTileM = 128, kBmmTileN = 256;
@@ -31,14 +33,14 @@ constexpr int kBmmABytes = kBmmTileM * 128;
 constexpr int kBmmStageBytes = kBmmABytes + kBmmTileN * 128;
 constexpr int kBmmScaleSlots = 2;         // ring of scale products, four K blocks a slot
 constexpr int kBmmScaleSlotFloats = 4 * 2 * kBmmTileM;
-constexpr int kBmmEpiPitch = 12;          // words: 16 bf16 columns of a row, padded (conflict-free 16-byte accesses)
+constexpr int kBmmEpiPitch = 8;           // words: 16 bf16 columns of a row
 constexpr int kBmmEpiBytes = kBmmEpiWarps * 32 * kBmmEpiPitch * 4;
 constexpr int kBmmMisc = 256;
 constexpr int kBmmSmemBytes = kBmmStages * kBmmStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
 static_assert(kBmmSmemBytes <= 227 * 1024, "shared memory budget");
-// setmaxnreg redistributes the 384 x 168 registers of the launch: what the roles take must not exceed it.
-constexpr int kBmmThinRegs = 56, kBmmFatRegs = 224;
-static_assert(128 * kBmmThinRegs + 256 * kBmmFatRegs <= kBmmThreads * 168, "register budget");
+// setmaxnreg redistributes the 512 x 128 registers of the launch: what the roles take must not exceed it.
+constexpr int kBmmThinRegs = 80, kBmmIssueRegs = 40, kBmmFatRegs = 184;
+static_assert(128 * (kBmmThinRegs + kBmmIssueRegs) + 256 * kBmmFatRegs <= kBmmThreads * 128, "register budget");
 
 enum : int { kStatusBmmTimeout = 0x600 };
 
@@ -111,8 +113,8 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   uint8_t* misc = smem + kBmmStages * kBmmStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(misc);
   uint64_t* empty_bar = full_bar + kBmmStages;
-  uint64_t* part_full_bar = empty_bar + kBmmStages;      // [half][2]
-  uint64_t* part_empty_bar = part_full_bar + 4;          // [half][2]
+  uint64_t* part_full_bar = empty_bar + kBmmStages;      // [half][parity]
+  uint64_t* part_empty_bar = part_full_bar + 4;          // [half][parity]
   uint64_t* sc_full_bar = part_empty_bar + 4;            // [kBmmScaleSlots]
   uint64_t* sc_empty_bar = sc_full_bar + kBmmScaleSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty_bar + kBmmScaleSlots);
@@ -176,44 +178,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       }
       if (!ok && lane == 0) bmm_fail(p.status, 0x01);
       ptx::pdl_release();
-    } else if (warp & 1) {
-      // ---------------------------------------------------------------- MMA issuers
-      // Warp 1 multiplies the tile's first 128 weight rows, warp 3 the other 128: each half has two
-      // accumulators and epilogue warps of its own, so a half-tile's round trip -- MMAs, commit, wake-up,
-      // drain, release -- overlaps the other half's.
-      const int half = warp >> 1;
-      const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
-      const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty0 = ptx::smem_u32(part_empty_bar) + 16 * half;
-      constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
-      const uint32_t smem0 = ptx::smem_u32(smem);
-      const uint64_t da0 = ptx::make_smem_desc(kDesc, smem0);
-      const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kBmmABytes + half * 128 * 128);
-      const uint32_t d_tmem = tmem_base + half * 256;
-      const int my_tiles = blockIdx.x < total_tiles ? (total_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
-      const long long stages = static_cast<long long>(my_tiles) * p.kb;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (long long it = 0; ok && it < stages; it += kBmmStages) {
-#pragma unroll
-        for (int st = 0; st < kBmmStages; ++st) {
-          if (it + st >= stages) break;
-          if (!ptx::mbar_wait(full0 + 8 * st, phase, abort_flag) ||
-              !ptx::mbar_wait(part_empty0 + 8 * (st & 1), ((st >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-          ptx::tc_fence_after();
-          if (ptx::elect_one()) {
-            constexpr uint32_t kStep = kBmmStageBytes >> 4;
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              ptx::umma_f8(d_tmem + (st & 1) * 128, da0 + (st * kStep + kk * 2), db0 + (st * kStep + kk * 2), p.idesc, kk ? 1u : 0u);
-            ptx::umma_commit(part_full0 + 8 * (st & 1));
-            ptx::umma_commit(empty0 + 8 * st);
-          }
-          __syncwarp();
-        }
-        phase ^= 1u;
-      }
-      if (!ok && lane == 0) bmm_fail(p.status, 0x02);
-    } else if (warp == 2) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------------- scale products
       int slot = 0;
       uint32_t sphase = 0;
@@ -264,53 +229,113 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       }
       if (!ok && lane == 0) bmm_fail(p.status, 0x03);
     }
+  } else if (warp < 8) {
+    ptx::setmaxnreg_dec<kBmmIssueRegs>();
+    // ------------------------------------------------------------------ MMA issuers
+    const int half = (warp >> 1) & 1, parity = warp & 1;
+    static_assert(kBmmStages == 4, "an issuer goes to and fro between two stages");
+    const uint32_t full0 = ptx::smem_u32(full_bar) + 8 * parity, empty0 = ptx::smem_u32(empty_bar) + 8 * parity;
+    const uint32_t part_full = ptx::smem_u32(part_full_bar) + 8 * (2 * half + parity), part_empty = ptx::smem_u32(part_empty_bar) + 8 * (2 * half + parity);
+    constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
+    const uint32_t smem0 = ptx::smem_u32(smem) + parity * kBmmStageBytes;
+    const uint64_t da0 = ptx::make_smem_desc(kDesc, smem0);
+    const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kBmmABytes + half * 128 * 128);
+    const uint32_t d_tmem = tmem_base + half * 256 + parity * 128;
+    const int my_tiles = blockIdx.x < total_tiles ? (total_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+    const long long stages = static_cast<long long>(my_tiles) * p.kb;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (long long it = parity; ok && it < stages; it += 4) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {             // stages parity and parity + 2
+        if (it + 2 * h >= stages) break;
+        if (!ptx::mbar_wait(full0 + 16 * h, phase, abort_flag) || !ptx::mbar_wait(part_empty, h ^ 1u, abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          constexpr uint32_t kTwo = (2 * kBmmStageBytes) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da0 + (h * kTwo + kk * 2), db0 + (h * kTwo + kk * 2), p.idesc, kk ? 1u : 0u);
+          ptx::umma_commit(part_full);
+          ptx::umma_commit(empty0 + 16 * h);
+        }
+        __syncwarp();
+      }
+      phase ^= 1u;
+    }
+    if (!ok && lane == 0) bmm_fail(p.status, 0x02);
   } else {
     // ------------------------------------------------------------------ promotion and epilogue
     ptx::setmaxnreg_inc<kBmmFatRegs>();
     const int quad = warp & 3;
-    const int half = (warp - 4) >> 2;                    // 128-column half: one weight block
-    uint32_t* mine = epi + (warp - 4) * (32 * kBmmEpiPitch);
+    const int half = (warp - 8) >> 2;
+    uint32_t* mine = epi + (warp - 8) * (32 * kBmmEpiPitch);
+    // x is the accumulator that the first and the third of four K blocks are in, y the other one.
     const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty0 = ptx::smem_u32(part_empty_bar) + 16 * half;
-    const uint32_t sc_full0 = ptx::smem_u32(sc_full_bar), sc_empty0 = ptx::smem_u32(sc_empty_bar);
-    const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 256);
-    const float* sc_base = sc_ring + half * kBmmTileM + quad * 32 + lane;
+    uint32_t full_x = part_full0, full_y = part_full0 + 8, empty_x = part_empty0, empty_y = part_empty0 + 8;
+    uint32_t t_x = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 256), t_y = t_x + 128;
+    uint32_t phase_x = 0, phase_y = 0;
+    static_assert(kBmmScaleSlots == 2, "the scale slots alternate");
+    uint32_t sc_full_now = ptx::smem_u32(sc_full_bar), sc_full_next = sc_full_now + 8;
+    uint32_t sc_empty_now = ptx::smem_u32(sc_empty_bar), sc_empty_next = sc_empty_now + 8;
+    int slot_now = 0, slot_next = kBmmScaleSlotFloats;
+    uint32_t sc_phase = 0;                               // of both slots: flips every two groups
     const int kb = p.kb, m_blocks = p.m_blocks;
-    uint32_t it = 0, group = 0;                          // stages and scale groups so far
+    const bool leader = lane == 0;
+    const float* sc_base = sc_ring + half * kBmmTileM + quad * 32 + lane;
     bool ok = true;
     for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
       const int m0 = tile % m_blocks * kBmmTileM, n0 = tile / m_blocks * kBmmTileN;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-      for (int k = 0; k < kb; ++k) {
-        if ((k & 3) == 0 && !ptx::mbar_wait(sc_full0 + 8 * (group % kBmmScaleSlots), (group / kBmmScaleSlots) & 1u, abort_flag)) { ok = false; break; }
-        const float sc = sc_base[(group % kBmmScaleSlots) * kBmmScaleSlotFloats + 2 * (k & 3) * kBmmTileM];
-        if (!ptx::mbar_wait(part_full0 + 8 * (it & 1u), (it >> 1) & 1u, abort_flag)) { ok = false; break; }
-        ptx::tc_fence_after();
-        const uint32_t t = t_base + (it & 1u) * 128;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kb; k0 += 4) {
+        if (!ptx::mbar_wait(sc_full_now, sc_phase, abort_flag)) { ok = false; break; }
+        float sc[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          ptx::tmem_ld_32x32(t + c * 32, v);
-          ptx::tmem_ld_wait();
-          if (c == 3) {
-            // everything has left this accumulator: the MMAs may overwrite it
-            ptx::tc_fence_before();
-            ptx::mbar_arrive_if(part_empty0 + 8 * (it & 1u), lane == 0);
-            ++it;
-            if ((k & 3) == 3 || k + 1 == kb) {
-              ptx::mbar_arrive_if(sc_empty0 + 8 * (group % kBmmScaleSlots), lane == 0);
-              ++group;
+        for (int u = 0; u < 4; ++u) sc[u] = sc_base[slot_now + 2 * u * kBmmTileM];
+        __syncwarp();
+        ptx::mbar_arrive_if(sc_empty_now, leader);
+        if (slot_now != 0) sc_phase ^= 1u;
+        const uint32_t f = sc_full_now, e = sc_empty_now;
+        const int sl = slot_now;
+        sc_full_now = sc_full_next; sc_full_next = f;
+        sc_empty_now = sc_empty_next; sc_empty_next = e;
+        slot_now = slot_next; slot_next = sl;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (k0 + u < kb) {
+            if (!ptx::mbar_wait((u & 1) ? full_y : full_x, (u & 1) ? phase_y : phase_x, abort_flag)) { ok = false; break; }
+            ptx::tc_fence_after();
+            const uint32_t t = (u & 1) ? t_y : t_x;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              ptx::tmem_ld_32x32(t + c * 32, v);
+              ptx::tmem_ld_wait();
+              if (c == 3) {      // everything has left this accumulator: the MMAs may overwrite it
+                ptx::tc_fence_before();
+                ptx::mbar_arrive_if((u & 1) ? empty_y : empty_x, leader);
+                if (u & 1) phase_y ^= 1u; else phase_x ^= 1u;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), sc[u], acc[c * 32 + j]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), sc, acc[c * 32 + j]);
         }
+        if (!ok) break;
+      }
+      if (kb & 1) {      // the next tile starts with the other accumulator
+        uint32_t x;
+        x = full_x; full_x = full_y; full_y = x;
+        x = empty_x; empty_x = empty_y; empty_y = x;
+        x = t_x; t_x = t_y; t_y = x;
+        x = phase_x; phase_x = phase_y; phase_y = x;
       }
       if (!ok) break;
       store_rows_bf16<128>(acc, mine, p.out, m0 + quad * 32, p.m, n0 + half * 128, p.n);
     }
-    if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x04);
+    if (!ok && threadIdx.x == 256) bmm_fail(p.status, 0x04);
   }
 
   ptx::tc_fence_before();
