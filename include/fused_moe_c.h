@@ -424,8 +424,9 @@ FMOE_API int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const int3
  *   out[i, j] = bf16( sum_b a_scale[i, b] w_scale[j / 128, b] sum_{k in block b} a[i, k] w[j, k] )
  * a [m, k] and a_scale as fmoe_quantise_rows writes them for `quant` (FMOE_QUANT_BLOCK128: f32
  * [m, k/128]; FMOE_QUANT_BLOCK128_UE8M0: bytes [m, roundup(k/128, 4)]), w [n, k], w_scale f32
- * [ceil(n/128), k/128] (powers of two for FMOE_QUANT_BLOCK128_UE8M0), out bf16 [m, n].  k is a
- * multiple of 128, m and n are any. */
+ * [ceil(n/128), k/128] (powers of two for FMOE_QUANT_BLOCK128_UE8M0: only the exponent is read), out
+ * bf16 [m, n].  k is a multiple of 128, m and n are any.  The kernel, and with it the order of the
+ * f32 sums, depends on m, n and k. */
 FMOE_API int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
                                   int32_t n, int32_t k, int32_t quant, void* out, int32_t* status, void* stream);
 

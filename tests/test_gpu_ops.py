@@ -262,6 +262,32 @@ def test_matmul_block128_special_values(m, quant):
     assert bool((raw[:4096] == 7).all()) and bool((raw[4096 + m * n:] == 7).all())
 
 
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_power_of_two_scales_at_their_limits(m):
+    """The smallest scale, the largest finite one and NaN; weight scales count by their exponent."""
+    n, k = 136, 256
+    a, sa, w, sw = block_inputs(m, n, k, "block128_ue8m0", seed=12)
+    sa[0, 0], sa[1, 1] = 0, 255
+    sw.fill_(1.0)
+    out = M.matmul_block128(a, sa, w, sw, "block128_ue8m0")
+    assert bool(torch.isnan(out[1]).all()) and not bool(torch.isnan(out[0]).any())
+    keep = [i for i in range(m) if i != 1]
+    ref, mag = block_reference(a[keep], sa[keep], w, sw, "block128_ue8m0")
+    close(out[keep], ref, (k + 8) * U * mag + 2.0 ** -110)
+    assert torch.equal(M.matmul_block128(a[keep], sa[keep], w, sw * 1.75, "block128_ue8m0"), out[keep])
+
+
+def test_every_kernel_of_the_product_is_reached():
+    """Rows from one to many: the tiles of 16, 32 and 128 rows with and without a split of K, and the
+    128 x 256 tiles, each against 64 bits (the choice goes by m, n and k)."""
+    for quant in ("block128", "block128_ue8m0"):
+        for m, n, k in ((1, 128, 128), (16, 384, 4096), (17, 2304, 4096), (40, 4096, 2048), (100, 7744, 1024), (130, 640, 1920), (70, 18432, 256), (520, 2048, 640)):
+            a, sa, w, sw = block_inputs(m, n, k, quant, seed=m)
+            ref, mag = block_reference(a, sa, w, sw, quant)
+            close(M.matmul_block128(a, sa, w, sw, quant), ref, (k + 8) * U * mag)
+    assert M.operator_status() == 0
+
+
 # ----------------------------------------------------------------------------- the gated activation
 def silu_reference(gu, weight, dy):
     g, u = gu.double().chunk(2, 1)
@@ -444,6 +470,57 @@ def test_a_captured_training_step():
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_results_given_by_the_caller():
+    off = offsets_of([3, 30])
+    x, w = torch.randn(33, 64, device=DEV).bfloat16(), torch.randn(2, 48, 64, device=DEV).bfloat16()
+    dy = torch.randn(33, 48, device=DEV).bfloat16()
+    gu, rw = torch.randn(9, 512, device=DEV).half(), torch.rand(9, device=DEV)
+    q = block_inputs(5, 70, 256, "block128", seed=2)
+    for call in (lambda **o: M.grouped_matmul(x, w, off, **o), lambda **o: M.grouped_matmul_dgrad(dy, w, off, **o),
+                 lambda **o: M.grouped_matmul_wgrad(dy, x, off, **o), lambda **o: M.silu_mul(gu, rw, **o), lambda **o: M.matmul_block128(*q, **o)):
+        want = call()
+        out = torch.empty_like(want)
+        assert call(out=out) is out and torch.equal(out, want)
+    qs, ss = M.silu_mul_quantise(gu, "block128", rw)
+    q2, s2 = torch.empty_like(qs), torch.empty_like(ss)
+    M.silu_mul_quantise(gu, "block128", rw, q=q2, scales=s2)
+    assert torch.equal(qs, q2) and torch.equal(ss, s2)
+
+
+def test_calls_from_a_thread_that_has_made_none():
+    """The first CUDA work of a thread: nothing has made the context current there yet."""
+    import threading
+    call, _ = _everything()
+    want, got = call(), []
+    torch.cuda.synchronize()
+    t = threading.Thread(target=lambda: got.extend(call()))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_two_threads_at_once():
+    import threading
+    call, _ = _everything()
+    want = call()
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        s = torch.cuda.Stream(DEV)
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got[i] = call()
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(want, g))
 
 
 def test_the_wrappers_refuse_what_does_not_fit():

@@ -172,7 +172,11 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     float s[2][kR][4], w[2][4];
     auto request = [&](int k, float (&sv)[kR][4], float (&wv)[4]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wv[j] = k + j < k1 ? __ldg(sw + k + j) : 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        wv[j] = k + j < k1 ? __ldg(sw + k + j) : 0.0f;
+        // power-of-two scales go by their exponent alone, as in the kernel whose MMAs apply them
+        if (kBytes) wv[j] = ue8m0_value((__float_as_uint(wv[j]) >> 23) & 0xffu);
+      }
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
         const int t = t0 + 32 * r + lane;
