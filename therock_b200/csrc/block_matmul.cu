@@ -117,7 +117,7 @@ int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p
 // estimated to be done first.  An estimate is a fixed part (launch, set-up, the way of the first blocks,
 // the result) and a time for each K block of the longest CTA, in nanoseconds, fitted to measured times of
 // 1 to 2048 rows times weights of 1024 x 1024 up to 18432 x 7168; over those the choice is 1.1 % from
-// the best on average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 and 1.5 times as many
+// the best on average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times as many
 // at the same time; with 128 rows there are whole rounds.
 int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
   const int64_t n_tiles = (n + 127) / 128;
@@ -125,7 +125,7 @@ int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& ro
   const int64_t big_tiles = (m + kBmmTileM - 1) / kBmmTileM * ((n + tile_n - 1) / tile_n);
   double best = (hw ? 4600.0 : 5000.0) + static_cast<double>((big_tiles + sms - 1) / sms) * kb * (hw ? 330.0 : 440.0);
   int choice = 0;
-  const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2400, 300, 1.6}, {32, 3500, 360, 1.5}, {128, 5500, 420, 1.0}};
+  const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2200, 300, 1.6}, {32, 3200, 360, 1.6}, {128, 6000, 420, 1.0}};
   for (const auto& kind : kinds) {
     const int64_t tiles = (m + kind.nt - 1) / kind.nt * n_tiles;
     if (tiles > (int64_t{1} << 20)) continue;

@@ -132,38 +132,47 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x11);
     ptx::pdl_release();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
+  } else if (warp & 1 && warp < 4) {
+    // ------------------------------------------------------------------ MMA issuers
+    // Two warps take turns, as a stage's waits, MMAs and commits keep one for longer than its MMAs take:
+    // this one has the blocks of one parity, and the accumulators of that parity.
+    const int mine = warp >> 1;
     const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar);
     const uint32_t part_full0 = ptx::smem_u32(part_full_bar), part_empty0 = ptx::smem_u32(part_empty_bar);
     constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
     const uint64_t da0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem));
     const uint64_t db0 = ptx::make_smem_desc(kDesc, ptx::smem_u32(smem) + kBsWBytes);
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, buf_phase = 0;
+    const int stages = p.stages;
+    int stage = mine;
+    uint32_t phase = 0, buf_phase = 1;
+    if (stage >= stages) { stage -= stages; phase = 1; }
     bool ok = true;
-    for (int k = k0; k < k1; ++k) {
-      if (!ptx::mbar_wait(full0 + 8 * stage, phase, abort_flag) ||
-          !ptx::mbar_wait(part_empty0 + 8 * buf, buf_phase ^ 1u, abort_flag)) { ok = false; break; }
-      ptx::tc_fence_after();
-      if (ptx::elect_one()) {
-        const uint64_t da = da0 + static_cast<uint32_t>(stage * (Cfg::kStageBytes >> 4));
-        const uint64_t db = db0 + static_cast<uint32_t>(stage * (Cfg::kStageBytes >> 4));
+    for (int k = k0 + mine; ok && k < k1; k += Cfg::kBufs) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(tmem_base + buf * kNT, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
-        ptx::umma_commit(part_full0 + 8 * buf);
-        ptx::umma_commit(empty0 + 8 * stage);
+      for (int h = 0; h < Cfg::kBufs; h += 2) {
+        if (k + h >= k1) break;
+        if (!ptx::mbar_wait(full0 + 8 * stage, phase, abort_flag) ||
+            !ptx::mbar_wait(part_empty0 + 8 * (mine + h), buf_phase, abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint64_t da = da0 + static_cast<uint32_t>(stage * (Cfg::kStageBytes >> 4));
+          const uint64_t db = db0 + static_cast<uint32_t>(stage * (Cfg::kStageBytes >> 4));
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(tmem_base + (mine + h) * kNT, da + kk * 2, db + kk * 2, p.idesc, kk ? 1u : 0u);
+          ptx::umma_commit(part_full0 + 8 * (mine + h));
+          ptx::umma_commit(empty0 + 8 * stage);
+        }
+        __syncwarp();
+        stage += 2;
+        while (stage >= stages) { stage -= stages; phase ^= 1u; }
       }
-      __syncwarp();
-      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
-      if (++buf == Cfg::kBufs) { buf = 0; buf_phase ^= 1u; }
+      buf_phase ^= 1u;
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x12);
-  } else if (warp < 4) {
+  } else if (warp == 2) {
     // ------------------------------------------------------------------ scale products
-    // Warps 2 and 3 take turns (slots of even and odd index).  Each requests its next slot before it
-    // hands over the present one: four slots, sixteen blocks of K, are on their way from the start, as
-    // a product of few blocks is over before a second round trip to memory.
+    // The next slot is requested before the present one is handed over: two slots, eight blocks of K, are
+    // on their way from the start.
     constexpr int kR = (kNT + 31) / 32;
     const uint32_t sc_full0 = ptx::smem_u32(sc_full_bar), sc_empty0 = ptx::smem_u32(sc_empty_bar);
     const float* sw = p.w_scale + static_cast<size_t>(n_blk) * p.kb;
@@ -204,7 +213,7 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       }
     };
     bool ok = true;
-    int n = warp - 2;                       // index of the slot's turn
+    int n = 0;                              // slots handed over
     auto hand_over = [&](int k, float (&sv)[kR][4], float (&wv)[4]) {
       const int slot = n % kBsScaleSlots;
       if (!ptx::mbar_wait(sc_empty0 + 8 * slot, ((n / kBsScaleSlots) & 1u) ^ 1u, abort_flag)) { ok = false; return; }
@@ -217,16 +226,16 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(sc_full0 + 8 * slot);
       __syncwarp();
-      n += 2;
+      ++n;
     };
-    int k = k0 + 4 * (warp - 2);
+    int k = k0;
     request(k, s[0], w[0]);
-    for (; ok && k < k1; k += 16) {
-      request(k + 8, s[1], w[1]);
+    for (; ok && k < k1; k += 8) {
+      request(k + 4, s[1], w[1]);
       hand_over(k, s[0], w[0]);
-      if (!ok || k + 8 >= k1) break;
-      request(k + 16, s[0], w[0]);
-      hand_over(k + 8, s[1], w[1]);
+      if (!ok || k + 4 >= k1) break;
+      request(k + 8, s[0], w[0]);
+      hand_over(k + 4, s[1], w[1]);
     }
     if (!ok && lane == 0) bmm_fail(p.status, 0x13);
   }
@@ -240,41 +249,48 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     const uint32_t part_full0 = ptx::smem_u32(part_full_bar), part_empty0 = ptx::smem_u32(part_empty_bar);
     const uint32_t sc_full0 = ptx::smem_u32(sc_full_bar), sc_empty0 = ptx::smem_u32(sc_empty_bar);
     const uint32_t t_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(col0);
-    int buf = 0, slot = 0;
-    uint32_t buf_phase = 0, sphase = 0;
+    const float* sc_base = sc_ring + col0;
+    int group = 0;
     bool ok = true;
 #pragma unroll
     for (int j = 0; j < Cfg::kCols; ++j) acc[j] = 0.0f;
-    for (int k = k0; k < k1; ++k) {
-      const int j4 = (k - k0) & 3;
-      if ((j4 == 0 && !ptx::mbar_wait(sc_full0 + 8 * slot, sphase, abort_flag)) ||
-          !ptx::mbar_wait(part_full0 + 8 * buf, buf_phase, abort_flag)) { ok = false; break; }
-      ptx::tc_fence_after();
-      const float4* sc = reinterpret_cast<const float4*>(sc_ring + (slot * 4 + j4) * kNT + col0);
-      // the whole accumulator is read before anything is added, so it is free again at once
-      uint32_t v[Cfg::kCols];
-      if constexpr (Cfg::kCols == 16) {
-        ptx::tmem_ld_32x16(t_base + buf * kNT, reinterpret_cast<uint32_t(&)[16]>(v[0]));
-      } else {
+    // four K blocks at a time: a slot of scales, and accumulators whose addresses do not change
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 4, ++group) {
+      const int slot = group % kBsScaleSlots, buf0 = (group * 4) % Cfg::kBufs;
+      const uint32_t phase = (group * 4 / Cfg::kBufs) & 1u;
+      if (!ptx::mbar_wait(sc_full0 + 8 * slot, (group / kBsScaleSlots) & 1u, abort_flag)) { ok = false; break; }
+      const float4* sc = reinterpret_cast<const float4*>(sc_base + slot * 4 * kNT);
 #pragma unroll
-        for (int c = 0; c < Cfg::kCols; c += 32) ptx::tmem_ld_32x32(t_base + buf * kNT + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
-      }
-      ptx::tmem_ld_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(part_empty0 + 8 * buf);
+      for (int u = 0; u < 4; ++u) {
+        if (k + u < k1) {
+          if (!ptx::mbar_wait(part_full0 + 8 * (buf0 + u), phase, abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          // the whole accumulator is read before anything is added, so it is free again at once
+          uint32_t v[Cfg::kCols];
+          const uint32_t t = t_base + (buf0 + u) * kNT;
+          if constexpr (Cfg::kCols == 16) {
+            ptx::tmem_ld_32x16(t, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+          } else {
 #pragma unroll
-      for (int q = 0; q < Cfg::kCols / 4; ++q) {
-        const float4 f = sc[q];
-        acc[4 * q] = fmaf(__uint_as_float(v[4 * q]), f.x, acc[4 * q]);
-        acc[4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), f.y, acc[4 * q + 1]);
-        acc[4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), f.z, acc[4 * q + 2]);
-        acc[4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), f.w, acc[4 * q + 3]);
+            for (int c = 0; c < Cfg::kCols; c += 32) ptx::tmem_ld_32x32(t + c, reinterpret_cast<uint32_t(&)[32]>(v[c]));
+          }
+          ptx::tmem_ld_wait();
+          ptx::tc_fence_before();
+          ptx::mbar_arrive_if(part_empty0 + 8 * (buf0 + u), lane == 0);
+#pragma unroll
+          for (int q = 0; q < Cfg::kCols / 4; ++q) {
+            const float4 f = sc[u * (kNT / 4) + q];
+            acc[4 * q] = fmaf(__uint_as_float(v[4 * q]), f.x, acc[4 * q]);
+            acc[4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), f.y, acc[4 * q + 1]);
+            acc[4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), f.z, acc[4 * q + 2]);
+            acc[4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), f.w, acc[4 * q + 3]);
+          }
+        }
       }
+      if (!ok) break;
       __syncwarp();
-      if (j4 == 3 && lane == 0) ptx::mbar_arrive(sc_empty0 + 8 * slot);
-      if (++buf == Cfg::kBufs) { buf = 0; buf_phase ^= 1u; }
-      if (j4 == 3 && ++slot == kBsScaleSlots) { slot = 0; sphase ^= 1u; }
+      ptx::mbar_arrive_if(sc_empty0 + 8 * slot, lane == 0);
     }
     if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x14);
   }
