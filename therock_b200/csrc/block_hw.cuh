@@ -11,6 +11,10 @@
 // A second accumulator would leave tensor memory no room for the scales.  When a tile is complete the
 // epilogue warps drain it into registers, hand tensor memory back and store while the next tile is
 // multiplied.
+//
+// Measured on a B200, 8192 x 4096 x 7168: 181 to 187 us = 2570 to 2660 TFLOP/s, what a library e4m3 product
+// without block scales sustains (2606) under the power limit that bounds both; the promotion in
+// registers took 250 us.
 #pragma once
 
 #include "block_matmul.cuh"

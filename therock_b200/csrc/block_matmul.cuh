@@ -14,6 +14,11 @@
 // of the stage), and the epilogue's loop takes four K blocks at a time with all addresses and parities in
 // registers.
 //
+// Measured on a B200, 8192 x 4096 x 7168: 219 us = 2193 TFLOP/s, 770 cycles a stage at the 1.6 GHz that the
+// power limit leaves; a library e4m3 product without block scales sustains 2606 there.  One issuing warp
+// and one 256-column accumulator per stage took 245 us, sixteen epilogue warps of 64 columns 272, and
+// 192-column tiles whose accumulator is read at once 246.
+//
 // A separate warp loads the scales of four blocks at a time, multiplies the activations' by those of the
 // tile's two weight blocks and leaves the products in shared memory.
 #pragma once

@@ -12,6 +12,11 @@
 // 2, 4 or 8 CTAs.  Each adds up its blocks, sends every CTA its share of the columns through
 // distributed shared memory, and sums the shares it received in the order of the ranks: one launch, no
 // workspace, the same bits every time.
+//
+// Measured on a B200: 16 x 18432 x 7168 in 23.5 us = 5650 GB/s (memory-bound: 88 % of a copy's rate, the
+// rest is launch and the first block's way), 1 x 4096 x 2048 in 3.6 us, 16 x 4096 x 7168 in 7.0 (four CTAs to
+// a tile; 8.7 with one 32-column-aligned share per CTA, whose sums one CTA in four did alone), 64 x 7744 x
+// 2048 in 7.6.  The kernel with 128 x 256 tiles took 9.7, 38, 25 and 10 us there.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -6,6 +6,8 @@
 //
 // All of them are bound by memory: 6 bytes a cell forward (16-bit types), 10 backward, 5 with the
 // e4m3 result.  Every thread moves 16-byte vectors (8 cells) of the gate half and of the up half.
+// Measured on a B200, 16384 x 2048 bf16: forward 31 us = 6460 GB/s, the rate of a copy; backward with
+// row weights 53 us = 6340 GB/s (a block of 256 threads to a row, one vector each, took 63).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
