@@ -398,11 +398,11 @@ FMOE_API int fmoe_ep_wait_combine(const int32_t* topk_ids, int32_t T, int32_t K,
 /* ---- Operators that an expert layer is built from when it is not one fmoe_run: training (with
  * gradients), other activations, dense layers beside the experts.  Asynchronous on `stream`; no
  * workspace, no device memory of their own, no host synchronisation; the same inputs give the same
- * bits (no atomics).  Matrices are row-major and dense, 16-byte aligned.  `status` (optional) is a
- * device int32 that receives a code if a bounded wait in a kernel runs out (the results are then
- * not valid); it is not cleared.  Without it the code goes to a word of the library's, one per
- * device, which fmoe_operator_status waits for, returns and clears.  No counterpart in the
- * reference operator. */
+ * bits (no atomics).  Matrices are row-major and dense, 16-byte aligned; other arrays have their
+ * type's alignment; results share no memory with inputs.  `status` (optional) is a device int32 that
+ * receives a code if a bounded wait in a kernel runs out (the results are then not valid); it is not
+ * cleared.  Without it the code goes to a word of the library's, one per device, which
+ * fmoe_operator_status waits for, returns and clears.  No counterpart in the reference operator. */
 FMOE_API int fmoe_operator_status(int32_t device, int32_t* status_out);
 
 

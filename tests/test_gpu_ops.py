@@ -637,3 +637,170 @@ def test_torch_ops_have_the_same_results_and_gradients():
     assert torch.equal(g, M.silu_mul_backward(x.detach(), dy[:, :32].contiguous())[0])
     q = block_inputs(5, 70, 256, "block128", seed=2)
     assert torch.equal(ns.matmul_block128(*q), M.matmul_block128(*q))
+
+
+# ----------------------------------------------------------------------------- calls that are easy to get wrong
+def _differentiable_calls():
+    import therock_b200.torch_op  # noqa: F401
+    ns = torch.ops.therock_b200
+    off = offsets_of([10, 0, 23])
+    x = torch.randn(33, 64, device=DEV).bfloat16()
+    w = torch.randn(3, 96, 64, device=DEV).bfloat16()
+    rw = torch.rand(33, device=DEV)
+    return {"grouped": ((x, w), lambda x, w: M.grouped_matmul(x, w, off)), "silu": ((x, rw), M.silu_mul),
+            "op_grouped": ((x, w), lambda x, w: ns.grouped_matmul(x, w, off)), "op_silu": ((x, rw), ns.silu_mul)}
+
+
+@pytest.mark.parametrize("name", ["grouped", "silu", "op_grouped", "op_silu"])
+def test_a_captured_backward_pass_beside_a_living_graph(name):
+    """A leaf's node lives as long as any graph of it does, on the stream that graph was recorded on; the
+    default stream cannot join a capture, so the pass is refused, and goes through once the graph is gone."""
+    leaves, f = _differentiable_calls()[name]
+    leaves = [t.requires_grad_() for t in leaves]
+
+    def step():
+        return torch.autograd.grad(f(*leaves), leaves, dy)
+    living = f(*leaves)
+    dy = torch.randn_like(living)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(g):
+            step()
+    want = torch.autograd.grad(living, leaves, dy)        # the eager graph is as good as before
+    del living, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_captured_backward_pass_beside_a_graph_of_a_side_stream():
+    leaves, f = _differentiable_calls()["grouped"]
+    leaves = [t.requires_grad_() for t in leaves]
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        living = f(*leaves)
+        dy = torch.randn_like(living)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        got = torch.autograd.grad(f(*leaves), leaves, dy)
+    g.replay()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(living, leaves, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("name", ["grouped", "silu"])
+def test_forward_mode_derivatives_are_refused(name):
+    import torch.autograd.forward_ad as fwd
+    (x, other), f = _differentiable_calls()[name]
+    with fwd.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f(fwd.make_dual(x, torch.ones_like(x)), other)
+
+
+def test_results_share_no_memory_with_inputs():
+    off = offsets_of([2, 2])
+    x, w = torch.zeros(4, 64, device=DEV).bfloat16(), torch.zeros(2, 64, 64, device=DEV).bfloat16()
+    q, s, sw = torch.zeros(4, 128, dtype=torch.uint8, device=DEV), torch.ones(4, 1, device=DEV), torch.ones(1, 1, device=DEV)
+    gu = torch.zeros(4, 256, device=DEV).half()
+    flat = gu.view(-1)
+    for call in (lambda: M.grouped_matmul(x, w, off, out=x), lambda: M.grouped_matmul(x, w, off, out=w[1, 60:]),
+                 lambda: M.grouped_matmul_dgrad(x, w, off, out=x), lambda: M.grouped_matmul_wgrad(w[0], w[1], off, out=w),
+                 lambda: M.silu_mul(gu, out=flat[512:].view(4, 128)),
+                 lambda: M.silu_mul_quantise(gu, "block128", q=flat[:256].view(torch.uint8).view(4, 128)),
+                 lambda: M.silu_mul_quantise(gu, "block128", q=q, scales=q.view(-1)[496:].view(4, 4)),
+                 lambda: M.matmul_block128(q, s, q, sw, out=q.view(-1)[:32].view(torch.bfloat16).view(4, 4))):
+        with pytest.raises(M.FmoeError, match="share"):
+            call()
+
+
+def test_results_of_more_than_two_to_the_31_elements():
+    """Row indices times widths that pass 32 bits: the first, the middle and the last rows."""
+    rows, n = 270000, 8192
+    at = torch.tensor([0, 1, 131071, 262143, 262144, 262145, rows - 2, rows - 1], device=DEV)
+    torch.manual_seed(11)
+    off = torch.tensor([0, 262145, rows - 1], dtype=torch.int32, device=DEV)     # and a last row of no group
+    x = torch.randn(rows, 8, device=DEV).bfloat16()
+    w = torch.randn(2, n, 8, device=DEV).bfloat16()
+    y = M.grouped_matmul(x, w, off)
+    xd, group = x[at].double(), (at >= 262145).long()
+    ref = torch.einsum("rk,rnk->rn", xd, w.double()[group])
+    mag = torch.einsum("rk,rnk->rn", xd.abs(), w.double().abs()[group])
+    ref[-1], mag[-1] = 0, 0
+    close(y[at], ref, (8 + 8) * U * mag)
+    # y as the gradient: its sums over 8192 columns and over the rows
+    dx = M.grouped_matmul_dgrad(y, w, off)
+    yd = y[at].double()
+    ref = torch.einsum("rn,rnk->rk", yd, w.double()[group])
+    mag = torch.einsum("rn,rnk->rk", yd.abs(), w.double().abs()[group])
+    close(dx[at], ref, (n + 8) * U * mag)
+    dw = M.grouped_matmul_wgrad(y, x, off)
+    lo, hi = 262145, rows - 1
+    yg, xg = y[lo:hi].double(), x[lo:hi].double()
+    close(dw[1], yg.T @ xg, (hi - lo + 8) * U * (yg.abs().T @ xg.abs()))
+    del dw, dx, yg
+    act = M.silu_mul(y)
+    g, u = y[at].double().chunk(2, dim=1)
+    slack = (12 + 1.173 * g.abs()) * U
+    close(act[at], g * torch.sigmoid(g) * u, slack * (g * torch.sigmoid(g) * u).abs() + 2.0 ** -140)
+    del y, act
+    a, sa, b, sb = block_inputs(rows, n, 128, "block128", seed=4)
+    out = M.matmul_block128(a, sa, b, sb)
+    ref, mag = block_reference(a[at], sa[at], b, sb, "block128")
+    close(out[at], ref, (128 + 8) * U * mag)
+
+
+def test_weights_of_more_than_two_to_the_31_elements():
+    groups, n, k = 520, 2048, 2056
+    torch.manual_seed(12)
+    w = torch.empty(groups, n, k, device=DEV, dtype=torch.bfloat16).normal_()
+    sizes = [0] * groups
+    sizes[0], sizes[511], sizes[519] = 3, 2, 20
+    off = offsets_of(sizes)
+    x, dy = torch.randn(25, k, device=DEV).bfloat16(), torch.randn(25, n, device=DEV).bfloat16()
+    spans = [(0, 0, 3), (511, 3, 5), (519, 5, 25)]
+    y, dx, dw = M.grouped_matmul(x, w, off), M.grouped_matmul_dgrad(dy, w, off), M.grouped_matmul_wgrad(dy, x, off)
+    for g, lo, hi in spans:
+        xd, dd, wd = x[lo:hi].double(), dy[lo:hi].double(), w[g].double()
+        close(y[lo:hi], xd @ wd.T, (k + 8) * U * (xd.abs() @ wd.abs().T))
+        close(dx[lo:hi], dd @ wd, (n + 8) * U * (dd.abs() @ wd.abs()))
+        close(dw[g], dd.T @ xd, (hi - lo + 8) * U * (dd.abs().T @ xd.abs()))
+    assert not bool(dw[1:511].any()) and not bool(dw[512:519].any())
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Set-up on a first call (attributes, occupancy) does not break a capture."""
+    import subprocess
+    import sys
+    text = """
+import torch, therock_b200 as M
+d = "cuda:0"
+torch.manual_seed(0)
+off = torch.tensor([0, 5, 33], dtype=torch.int32, device=d)
+x, w = torch.randn(33, 64, device=d).bfloat16(), torch.randn(2, 256, 64, device=d).bfloat16()
+a, b = torch.randn(33, 256, device=d).to(torch.float8_e4m3fn), torch.randn(70, 256, device=d).to(torch.float8_e4m3fn)
+sa, sb = torch.rand(33, 2, device=d), torch.rand(1, 2, device=d)
+def calls():
+    gu = M.grouped_matmul(x, w, off)
+    y = M.silu_mul(gu)
+    q, s = M.silu_mul_quantise(gu, "block128")
+    dx, dw = M.grouped_matmul_dgrad(gu, w, off), M.grouped_matmul_wgrad(gu, x, off)
+    return gu, y, q, s, dx, dw, M.matmul_block128(a, sa, b, sb)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, calls()))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]

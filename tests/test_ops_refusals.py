@@ -94,3 +94,23 @@ def test_wrappers_refuse_host_tensors(lib):
                  lambda: M.matmul_block128(q, torch.zeros(4, 1), q, torch.zeros(1, 1), quant="token_channel")):
         with pytest.raises(M.FmoeError):
             call()
+
+
+def test_pointers_below_their_types_alignment_are_refused(lib):
+    assert lib.fmoe_grouped_matmul(P, P, P + 2, 4, 2, 64, 64, 0, 0, P, None, None) == -1
+    assert lib.fmoe_grouped_matmul(P, P, P, 4, 2, 64, 64, 0, 0, P, P + 1, None) == -1
+    assert lib.fmoe_grouped_matmul_wgrad(P, P, P + 1, 4, 2, 64, 64, 0, P, None, None) == -1
+    assert lib.fmoe_grouped_matmul_wgrad(P, P, P, 4, 2, 64, 64, 0, P, P + 2, None) == -1
+    assert lib.fmoe_matmul_block128(P, P, P, P, 3, 40, 256, 2, P, P + 2, None) == -1
+    assert lib.fmoe_silu_mul(P, P + 2, 3, 64, 0, P, None) == -1
+    assert lib.fmoe_silu_mul_quantise(P, P + 1, 3, 128, 0, 3, P, P, None) == -1
+    assert lib.fmoe_silu_mul_backward(P, P + 2, P, 3, 64, 0, P, P, None) == -1
+    assert lib.fmoe_silu_mul_backward(P, P, P, 3, 64, 0, P, P + 2, None) == -1
+    assert b"aligned" in lib.fmoe_last_error()
+
+
+def test_sizes_past_32_bits_are_refused(lib):
+    from therock_b200 import ops
+    with pytest.raises(ops.FmoeError):
+        ops._sizes(8, 2 ** 32 + 8)
+    ops._sizes(2 ** 31 - 1)

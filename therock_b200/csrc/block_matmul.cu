@@ -1,4 +1,7 @@
 // Host side of the e4m3 product with block scales: checks, tensor maps, launch.
+#include <atomic>
+#include <mutex>
+
 #include "block_hw.cuh"
 #include "block_small.cuh"
 
@@ -40,12 +43,12 @@ struct ClusterRoom {
 template <int kNT, bool kBytes>
 cudaError_t small_kernel_room(ClusterRoom* room) {
   static ClusterRoom known[kMaxDevices];
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices] = {};
   auto kernel = fmoe_matmul_block128_small_kernel<kNT, kBytes>;
   int dev = 0;
   cudaGetDevice(&dev);
   const bool cached = dev >= 0 && dev < kMaxDevices;
-  if (cached && configured[dev]) {
+  if (cached && configured[dev].load(std::memory_order_acquire)) {
     *room = known[dev];
     return cudaSuccess;
   }
@@ -64,8 +67,10 @@ cudaError_t small_kernel_room(ClusterRoom* room) {
     e = cudaOccupancyMaxActiveClusters(&room->most[i], kernel, &cfg);
   }
   if (e == cudaSuccess && cached) {
-    known[dev] = *room;
-    configured[dev] = true;
+    static std::mutex once;
+    std::lock_guard<std::mutex> lock(once);
+    if (!configured[dev].load(std::memory_order_relaxed)) known[dev] = *room;
+    configured[dev].store(true, std::memory_order_release);
   }
   return e;
 }
@@ -163,8 +168,9 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   if (!a || !a_scale || !w || !w_scale || !out)
     return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: a, a_scale, w, w_scale and out are required");
   auto misaligned = [](const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; };
-  if (misaligned(a, 15) || misaligned(w, 15) || misaligned(out, 15) || misaligned(a_scale, 3) || misaligned(w_scale, 3))
-    return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: a, w and out must be 16-byte aligned, the scales 4-byte aligned");
+  if (misaligned(a, 15) || misaligned(w, 15) || misaligned(out, 15) || misaligned(a_scale, 3) || misaligned(w_scale, 3) ||
+      misaligned(status, 3))
+    return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: a, w and out must be 16-byte aligned, the scales and status 4-byte aligned");
   DeviceGuard guard(a);
   if (guard.rc() != FMOE_OK) return guard.rc();
   NvtxRange range("fmoe_matmul_block128");

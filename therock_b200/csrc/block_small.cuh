@@ -15,8 +15,8 @@
 //
 // Measured on a B200: 16 x 18432 x 7168 in 23.5 us = 5650 GB/s (memory-bound: 88 % of a copy's rate, the
 // rest is launch and the first block's way), 1 x 4096 x 2048 in 3.6 us, 16 x 4096 x 7168 in 7.0 (four CTAs to
-// a tile; 8.7 with one 32-column-aligned share per CTA, whose sums one CTA in four did alone), 64 x 7744 x
-// 2048 in 7.6.  The kernel with 128 x 256 tiles took 9.7, 38, 25 and 10 us there.
+// a tile), 64 x 7744 x 2048 in 7.6.  The kernels with 128 x 256 tiles take 36 to 40 us for the first of these
+// shapes, 22 to 26 for the third and 8.5 to 10 for the last.
 #pragma once
 
 #include <cuda_bf16.h>

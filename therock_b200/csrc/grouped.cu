@@ -10,9 +10,13 @@ namespace {
 constexpr int kMaxDevices = 64;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
-int check_grouped(const char* name, const int32_t* offsets, int64_t rows, int32_t groups, int32_t n, int32_t k, int32_t dtype) {
+int check_grouped(const char* name, const int32_t* offsets, int64_t rows, int32_t groups, int32_t n, int32_t k, int32_t dtype,
+                  const int32_t* status) {
   if (!offsets) return fail(FMOE_ERR_INVALID_ARG, "%s: offsets are required", name);
+  if (!aligned4(offsets) || !aligned4(status))
+    return fail(FMOE_ERR_INVALID_ARG, "%s: offsets and status must be 4-byte aligned", name);
   if (rows < 0 || groups <= 0 || n <= 0 || k <= 0)
     return fail(FMOE_ERR_INVALID_ARG, "%s: bad dimensions (rows=%lld groups=%d n=%d k=%d)", name, (long long)rows, groups, n, k);
   if (dtype != FMOE_BF16 && dtype != FMOE_F16) return fail(FMOE_ERR_UNSUPPORTED, "%s: bf16 and f16 only", name);
@@ -88,7 +92,7 @@ extern "C" int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* 
                                    int32_t n, int32_t k, int32_t dtype, int32_t transpose_w, void* out, int32_t* status,
                                    void* stream_v) {
   using namespace fmoe;
-  int rc = check_grouped("fmoe_grouped_matmul", offsets, rows, groups, n, k, dtype);
+  int rc = check_grouped("fmoe_grouped_matmul", offsets, rows, groups, n, k, dtype, status);
   if (rc != FMOE_OK) return rc;
   if (transpose_w != 0 && transpose_w != 1) return fail(FMOE_ERR_INVALID_ARG, "fmoe_grouped_matmul: transpose_w must be 0 or 1");
   if (rows == 0) return FMOE_OK;
@@ -126,7 +130,7 @@ extern "C" int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* 
 extern "C" int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const int32_t* offsets, int64_t rows, int32_t groups,
                                          int32_t n, int32_t k, int32_t dtype, void* dw, int32_t* status, void* stream_v) {
   using namespace fmoe;
-  int rc = check_grouped("fmoe_grouped_matmul_wgrad", offsets, rows, groups, n, k, dtype);
+  int rc = check_grouped("fmoe_grouped_matmul_wgrad", offsets, rows, groups, n, k, dtype, status);
   if (rc != FMOE_OK) return rc;
   if (!dw || (rows > 0 && (!dy || !x))) return fail(FMOE_ERR_INVALID_ARG, "fmoe_grouped_matmul_wgrad: dy, x and dw are required");
   if (!aligned16(dy) || !aligned16(x) || !aligned16(dw))

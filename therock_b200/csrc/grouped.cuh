@@ -25,7 +25,7 @@
 // What it took: roles that run as whole warps with one elected thread (a lane-0 branch made the issue of
 // the MMAs and the loads the bound: 1.75 -> 1.31 ms), a store phase without a branch per store (-> 1.21), and
 // no cluster-scope release in a loop (dw 0.76 -> 0.49).  Prefetching the weights into L2 seven to sixteen
-// stages ahead made all of them 3 to 8 % slower.
+// stages ahead made y 3 to 9 % slower.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -278,8 +278,9 @@ silu_mul_backward_weighted_kernel(const uint4* __restrict__ gu, const float* __r
   }
 }
 
-int check_silu(const char* name, const void* gu, int64_t rows, int32_t width, int32_t dtype) {
+int check_silu(const char* name, const void* gu, const float* row_weight, int64_t rows, int32_t width, int32_t dtype) {
   if (!gu) return fail(FMOE_ERR_INVALID_ARG, "%s: gu is required", name);
+  if (reinterpret_cast<uintptr_t>(row_weight) & 3) return fail(FMOE_ERR_INVALID_ARG, "%s: row_weight must be 4-byte aligned", name);
   if (rows < 0 || width <= 0) return fail(FMOE_ERR_INVALID_ARG, "%s: bad dimensions (rows=%lld width=%d)", name, (long long)rows, width);
   if (dtype != FMOE_BF16 && dtype != FMOE_F16) return fail(FMOE_ERR_UNSUPPORTED, "%s: bf16 and f16 only", name);
   if (width % 8) return fail(FMOE_ERR_UNSUPPORTED, "%s: width must be a multiple of 8", name);
@@ -360,7 +361,7 @@ extern "C" int fmoe_silu_mul(const void* gu, const float* row_weight, int64_t ro
                              void* stream) {
   using namespace fmoe;
   if (rows == 0 && width > 0) return FMOE_OK;
-  int rc = check_silu("fmoe_silu_mul", gu, rows, width, dtype);
+  int rc = check_silu("fmoe_silu_mul", gu, row_weight, rows, width, dtype);
   if (rc != FMOE_OK) return rc;
   if (!out) return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul: out is required");
   if (!aligned16(gu) || !aligned16(out)) return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul: gu and out must be 16-byte aligned");
@@ -378,7 +379,7 @@ extern "C" int fmoe_silu_mul_quantise(const void* gu, const float* row_weight, i
   if (quant != FMOE_QUANT_BLOCK128 && quant != FMOE_QUANT_BLOCK128_UE8M0)
     return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_quantise: quant must be a block mode");
   if (rows == 0 && width > 0) return FMOE_OK;
-  int rc = check_silu("fmoe_silu_mul_quantise", gu, rows, width, dtype);
+  int rc = check_silu("fmoe_silu_mul_quantise", gu, row_weight, rows, width, dtype);
   if (rc != FMOE_OK) return rc;
   if (width % 128) return fail(FMOE_ERR_UNSUPPORTED, "fmoe_silu_mul_quantise: width must be a multiple of 128");
   if (!q || !scales) return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_quantise: q and scales are required");
@@ -397,13 +398,13 @@ extern "C" int fmoe_silu_mul_backward(const void* gu, const float* row_weight, c
                                       int32_t dtype, void* dgu, float* dweight, void* stream) {
   using namespace fmoe;
   if (rows == 0 && width > 0) return FMOE_OK;
-  int rc = check_silu("fmoe_silu_mul_backward", gu, rows, width, dtype);
+  int rc = check_silu("fmoe_silu_mul_backward", gu, row_weight, rows, width, dtype);
   if (rc != FMOE_OK) return rc;
   if (!dy || !dgu) return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_backward: dy and dgu are required");
   if ((row_weight != nullptr) != (dweight != nullptr))
     return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_backward: row_weight and dweight come together");
-  if (!aligned16(gu) || !aligned16(dy) || !aligned16(dgu))
-    return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_backward: gu, dy and dgu must be 16-byte aligned");
+  if (!aligned16(gu) || !aligned16(dy) || !aligned16(dgu) || (reinterpret_cast<uintptr_t>(dweight) & 3))
+    return fail(FMOE_ERR_INVALID_ARG, "fmoe_silu_mul_backward: gu, dy and dgu must be 16-byte aligned, dweight 4-byte aligned");
   DeviceGuard guard(gu);
   if (guard.rc() != FMOE_OK) return guard.rc();
   NvtxRange range("fmoe_silu_mul_backward");

@@ -6,10 +6,13 @@
 //
 // A function returns its result, or None where its arguments do not fit: ops.py then says what is wrong.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include "../../include/fused_moe_c.h"
@@ -46,6 +49,40 @@ void check(int rc) {
   if (rc != FMOE_OK) throw Failure(rc, F.last_error());
 }
 
+// The interpreter's lock is not held while a call allocates and launches: either may wait for the GPU.
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+bool fits32(const at::Tensor& t) {
+  for (const int64_t d : t.sizes())
+    if (d > INT32_MAX) return false;
+  return true;
+}
+bool differentiable(const at::Tensor& t) { return t.requires_grad() || t._fw_grad(0).defined(); }
+
+// A backward pass that is being captured cannot hand gradients to a node of the default stream, which
+// cannot join a capture: a leaf has such a node as long as any earlier graph of it lives.  The engine
+// would break the capture, and with it the process; this ends the pass with an error instead.
+void refuse_default_stream_in_capture(int device) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::Stream blocked = c10::cuda::getDefaultCUDAStream(static_cast<c10::DeviceIndex>(device)).unwrap();
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    const std::optional<c10::Stream> s = edge.function->stream();
+    if (s && *s == blocked)
+      throw std::runtime_error(
+          "a backward pass is being captured in a CUDA graph while an earlier graph of the same tensors, recorded "
+          "on the default stream, is alive: drop its results (or record it on a side stream) before the capture");
+  }
+}
+
 // A gradient that autograd may hand over with any strides, as the kernels read it.
 at::Tensor for_kernel(const at::Tensor& t) {
   at::Tensor c = t.contiguous();
@@ -70,7 +107,7 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
 
 // ----------------------------------------------------------------------------- products grouped by expert
 bool grouped_fits(const at::Tensor& x, const at::Tensor& w, const at::Tensor& off) {
-  return dense(x) && dense(w) && dense(off, 4) && half_type(x.scalar_type()) && w.scalar_type() == x.scalar_type() &&
+  return dense(x) && dense(w) && dense(off, 4) && fits32(w) && half_type(x.scalar_type()) && w.scalar_type() == x.scalar_type() &&
          off.scalar_type() == at::kInt && x.dim() == 2 && w.dim() == 3 && off.dim() == 1 && w.size(2) == x.size(1) &&
          off.size(0) == w.size(0) + 1 && w.get_device() == x.get_device() && off.get_device() == x.get_device();
 }
@@ -91,6 +128,7 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &off = saved[2];
+    refuse_default_stream_in_capture(x.get_device());
     torch::autograd::variable_list out(3);
     {
       at::NoGradGuard no_grad;
@@ -109,7 +147,9 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
 
 // ----------------------------------------------------------------------------- the gated activation
 bool silu_fits(const at::Tensor& gu, const std::optional<at::Tensor>& weight) {
-  if (!(dense(gu) && half_type(gu.scalar_type()) && gu.dim() == 2 && gu.size(1) % 16 == 0 && gu.size(1) > 0)) return false;
+  if (!(dense(gu) && half_type(gu.scalar_type()) && gu.dim() == 2 && gu.size(1) % 16 == 0 && gu.size(1) > 0 &&
+        gu.size(1) <= INT32_MAX))
+    return false;
   return !weight || (dense(*weight, 4) && weight->scalar_type() == at::kFloat && weight->dim() == 1 &&
                      weight->size(0) == gu.size(0) && weight->get_device() == gu.get_device());
 }
@@ -130,6 +170,7 @@ struct SiluMul : torch::autograd::Function<SiluMul> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &gu = saved[0], &weight = saved[1];
+    refuse_default_stream_in_capture(gu.get_device());
     torch::autograd::variable_list out(2);
     {
       at::NoGradGuard no_grad;
@@ -163,9 +204,13 @@ PyObject* py_grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *x, *w, *off;
   if (n != 3 || !(x = tensor(args[0])) || !(w = tensor(args[1])) || !(off = tensor(args[2])) || !grouped_fits(*x, *w, *off))
     Py_RETURN_NONE;
-  if (at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad()))
-    return THPVariable_Wrap(GroupedMatmul::apply(*x, *w, *off));
-  return THPVariable_Wrap(grouped(*x, *w, *off, false));
+  at::Tensor out;
+  {
+    Unlocked unlocked;
+    out = at::GradMode::is_enabled() && (differentiable(*x) || differentiable(*w)) ? GroupedMatmul::apply(*x, *w, *off)
+                                                                                   : grouped(*x, *w, *off, false);
+  }
+  return THPVariable_Wrap(std::move(out));
   FMOE_CATCH
 }
 
@@ -184,11 +229,15 @@ PyObject* py_matmul_block128(PyObject*, PyObject* const* args, Py_ssize_t n) {
       sa->size(1) != (bytes ? row_bytes : kb) || sw->scalar_type() != at::kFloat || sw->size(0) != (nn + 127) / 128 || sw->size(1) != kb ||
       sa->get_device() != a->get_device() || w->get_device() != a->get_device() || sw->get_device() != a->get_device())
     Py_RETURN_NONE;
-  at::Tensor out = at::empty({m, nn}, a->options().dtype(at::kBFloat16).requires_grad(false));
-  check(F.block128(a->data_ptr(), sa->data_ptr(), w->data_ptr(), sw->data_ptr<float>(), m, static_cast<int32_t>(nn),
-                   static_cast<int32_t>(k), hw ? FMOE_QUANT_BLOCK128_UE8M0 : FMOE_QUANT_BLOCK128, out.data_ptr(),
-                   nullptr, stream_of(*a)));
-  return THPVariable_Wrap(out);
+  at::Tensor out;
+  {
+    Unlocked unlocked;
+    out = at::empty({m, nn}, a->options().dtype(at::kBFloat16).requires_grad(false));
+    check(F.block128(a->data_ptr(), sa->data_ptr(), w->data_ptr(), sw->data_ptr<float>(), m, static_cast<int32_t>(nn),
+                     static_cast<int32_t>(k), hw ? FMOE_QUANT_BLOCK128_UE8M0 : FMOE_QUANT_BLOCK128, out.data_ptr(),
+                     nullptr, stream_of(*a)));
+  }
+  return THPVariable_Wrap(std::move(out));
   FMOE_CATCH
 }
 
@@ -205,9 +254,13 @@ PyObject* py_silu_mul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* gu;
   std::optional<at::Tensor> weight;
   if (n != 2 || !(gu = tensor(args[0])) || !weight_of(args[1], &weight) || !silu_fits(*gu, weight)) Py_RETURN_NONE;
-  if (at::GradMode::is_enabled() && (gu->requires_grad() || (weight && weight->requires_grad())))
-    return THPVariable_Wrap(SiluMul::apply(*gu, weight));
-  return THPVariable_Wrap(silu(*gu, weight));
+  at::Tensor out;
+  {
+    Unlocked unlocked;
+    out = at::GradMode::is_enabled() && (differentiable(*gu) || (weight && differentiable(*weight))) ? SiluMul::apply(*gu, weight)
+                                                                                                    : silu(*gu, weight);
+  }
+  return THPVariable_Wrap(std::move(out));
   FMOE_CATCH
 }
 
@@ -220,14 +273,27 @@ PyObject* py_silu_mul_quantise(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool hw = PyLong_AsLong(args[1]) == FMOE_QUANT_BLOCK128_UE8M0;
   const int64_t rows = gu->size(0), width = gu->size(1) / 2, groups = width / 128;
   const auto options = gu->options().dtype(at::kByte).requires_grad(false);
-  at::Tensor q = at::empty({rows, width}, options), scales = at::empty({rows, hw ? (groups + 3) / 4 * 4 : 4 * groups}, options);
-  check(F.silu_quantise(gu->data_ptr(), weight_ptr(weight), rows, static_cast<int32_t>(width), dtype_code(*gu),
-                        hw ? FMOE_QUANT_BLOCK128_UE8M0 : FMOE_QUANT_BLOCK128, q.data_ptr(), scales.data_ptr(), stream_of(*gu)));
+  at::Tensor q, scales;
+  {
+    Unlocked unlocked;
+    q = at::empty({rows, width}, options);
+    scales = at::empty({rows, hw ? (groups + 3) / 4 * 4 : 4 * groups}, options);
+    check(F.silu_quantise(gu->data_ptr(), weight_ptr(weight), rows, static_cast<int32_t>(width), dtype_code(*gu),
+                          hw ? FMOE_QUANT_BLOCK128_UE8M0 : FMOE_QUANT_BLOCK128, q.data_ptr(), scales.data_ptr(), stream_of(*gu)));
+  }
   PyObject* both = PyTuple_New(2);
   if (both == nullptr) return nullptr;
   PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(q));
   PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(scales));
   return both;
+  FMOE_CATCH
+}
+
+// For the backward of a node recorded in Python, on the current stream's device.
+PyObject* py_check_capture(PyObject*, PyObject*) {
+  FMOE_TRY
+  refuse_default_stream_in_capture(c10::cuda::current_device());
+  Py_RETURN_NONE;
   FMOE_CATCH
 }
 
@@ -265,6 +331,7 @@ PyMethodDef kMethods[] = {{"bind", FAST(py_bind), METH_FASTCALL, nullptr},
                           {"matmul_block128", FAST(py_matmul_block128), METH_FASTCALL, nullptr},
                           {"silu_mul", FAST(py_silu_mul), METH_FASTCALL, nullptr},
                           {"silu_mul_quantise", FAST(py_silu_mul_quantise), METH_FASTCALL, nullptr},
+                          {"check_capture", py_check_capture, METH_NOARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fmoe_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

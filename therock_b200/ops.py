@@ -8,7 +8,8 @@
 `grouped_matmul` and `silu_mul` have gradients (first order, through torch.autograd).  Every call
 enqueues kernels of libfmoe_b200.so on `stream` (the tensors' current stream by default) and
 returns: no host synchronisation, no atomics, so the same inputs give the same bits, and a call can
-be captured in a CUDA graph.  Inputs are contiguous CUDA tensors on one device, which need not be
+be captured in a CUDA graph (a forward and its backward pass in one graph; no earlier graph of the
+same tensors that was recorded on the default stream may be alive).  Inputs are contiguous CUDA tensors on one device, which need not be
 the current one; a call on another stream than the current one allocates its results for that
 stream, and the caller orders the streams.  Bad arguments raise FmoeError before any launch."""
 from __future__ import annotations
@@ -102,12 +103,23 @@ def _dense(name: str, t, device: int = -1, align: int = 16) -> int:
     return index
 
 
-def _result(name: str, out, shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
+def _sizes(*sizes) -> None:
+    """The entry points take these as 32-bit numbers."""
+    if max(sizes) > 0x7fffffff:
+        raise FmoeError(-2, "problem too large: all sizes but the number of rows must fit 32 bits")
+
+
+def _result(name: str, out, shape, dtype, like: torch.Tensor, stream, *apart) -> torch.Tensor:
+    """The tensor that takes the result; `apart` are those it must not share memory with."""
     if out is None:
         return _empty(shape, dtype, like, stream)
     _dense(name, out, like.get_device())
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise FmoeError(-1, f"{name} must be {dtype} {tuple(shape)}")
+    first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for t in apart:
+        if t is not None and t.data_ptr() < last and first < t.data_ptr() + t.numel() * t.element_size():
+            raise FmoeError(-1, f"{name} must not share memory with the other tensors")
     return out
 
 
@@ -139,7 +151,8 @@ def _check_grouped(x, weight, offsets):
 def _grouped(x, weight, offsets, transpose: bool, out, stream):
     groups, n, k = weight.shape
     rows = x.shape[0]
-    out = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream)
+    _sizes(groups, n, k)
+    out = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream, x, weight, offsets)
     rc = _bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), rows, groups, n, k, _DTYPE[x.dtype],
                                       transpose, out.data_ptr(), None, _stream_of(x, stream))
     if rc:
@@ -150,7 +163,7 @@ def _grouped(x, weight, offsets, transpose: bool, out, stream):
 def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
                          stream=None) -> torch.Tensor:
     """dx [rows, k] with dx[r] = weight[g]^T dy[r] for the rows of group g, zeros for rows of none: the
-    gradient of grouped_matmul with respect to x, from dy [rows, n]."""
+    gradient of grouped_matmul with respect to x, from dy [rows, n].  No gradient of its own."""
     index = _dense("dy", dy)
     _dense("weight", weight, index)
     _dense("offsets", offsets, index, 4)
@@ -166,7 +179,7 @@ def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.
 def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
                          stream=None) -> torch.Tensor:
     """dw [groups, n, k] with dw[g] = dy[rows of g]^T x[rows of g]; zeros for a group without rows.
-    Rows of no group do not enter it, whatever they hold."""
+    Rows of no group do not enter it, whatever they hold.  No gradient of its own."""
     index = _dense("dy", dy)
     _dense("x", x, index)
     _dense("offsets", offsets, index, 4)
@@ -177,7 +190,8 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2:
         raise FmoeError(-1, "offsets must be int32 [groups + 1]")
     groups, n, k = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
-    out = _result("out", out, (groups, n, k), x.dtype, x, stream)
+    _sizes(groups, n, k)
+    out = _result("out", out, (groups, n, k), x.dtype, x, stream, dy, x, offsets)
     _check(_bound().fmoe_grouped_matmul_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
                                               _DTYPE[x.dtype], out.data_ptr(), None, _stream_of(x, stream)))
     return out
@@ -211,7 +225,7 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     returns them, or a_scale as float32 [m, k/128] for "block128"; w [n, k] e4m3 and w_scale float32
     [ceil(n/128), k/128] (powers of two for "block128_ue8m0").  Each block's products are summed in 32
     bits and scaled by both scales before blocks are added, in 32 bits; one rounding.  k is a multiple
-    of 128, m and n are any."""
+    of 128, m and n are any.  No gradient."""
     if quant not in _BLOCK_QUANT:
         raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
     if out is None and stream is None:
@@ -238,7 +252,8 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
         raise FmoeError(-1, f"a_scale must hold {row_bytes} bytes for each of the {m} rows, as quantise_rows returns them")
     if w_scale.dtype is not torch.float32 or w_scale.shape != ((n + 127) // 128, blocks):
         raise FmoeError(-1, f"w_scale must be float32 [{(n + 127) // 128}, {blocks}]")
-    out = _result("out", out, (m, n), torch.bfloat16, a, stream)
+    _sizes(n, k)
+    out = _result("out", out, (m, n), torch.bfloat16, a, stream, a, a_scale, w, w_scale)
     _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
                                          QUANT[quant], out.data_ptr(), None, _stream_of(a, stream)))
     return out
@@ -255,19 +270,20 @@ def _check_silu(gu, row_weight):
         _dense("row_weight", row_weight, index, 4)
         if row_weight.dtype is not torch.float32 or row_weight.shape != gu.shape[:1]:
             raise FmoeError(-1, "row_weight must be float32 [rows]")
+    _sizes(gu.shape[1])
     return gu.shape[0], gu.shape[1] // 2
 
 
 def _silu(gu, row_weight, out, stream):
     rows, width = gu.shape[0], gu.shape[1] // 2
-    out = _result("out", out, (rows, width), gu.dtype, gu, stream)
+    out = _result("out", out, (rows, width), gu.dtype, gu, stream, gu, row_weight)
     _check(_bound().fmoe_silu_mul(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
                                   _DTYPE[gu.dtype], out.data_ptr(), _stream_of(gu, stream)))
     return out
 
 
 def silu_mul_backward(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optional[torch.Tensor] = None, stream=None):
-    """Gradients of silu_mul: (dgu [rows, 2 * width], dweight float32 [rows] or None)."""
+    """Gradients of silu_mul: (dgu [rows, 2 * width], dweight float32 [rows] or None).  No gradients of their own."""
     rows, width = _check_silu(gu, row_weight)
     _dense("dy", dy, gu.get_device())
     if dy.dtype != gu.dtype or tuple(dy.shape) != (rows, width):
@@ -310,8 +326,8 @@ def silu_mul_quantise(gu: torch.Tensor, quant: str, row_weight: Optional[torch.T
         raise FmoeError(-2, "width must be a multiple of 128")
     groups = width // 128
     row_bytes = 4 * groups if quant == "block128" else (groups + 3) // 4 * 4
-    q = _result("q", q, (rows, width), torch.uint8, gu, stream)
-    scales = _result("scales", scales, (rows, row_bytes), torch.uint8, gu, stream)
+    q = _result("q", q, (rows, width), torch.uint8, gu, stream, gu, row_weight)
+    scales = _result("scales", scales, (rows, row_bytes), torch.uint8, gu, stream, gu, row_weight, q)
     _check(_bound().fmoe_silu_mul_quantise(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
                                            _DTYPE[gu.dtype], QUANT[quant], q.data_ptr(), scales.data_ptr(),
                                            _stream_of(gu, stream)))

@@ -72,12 +72,20 @@ def _(dy, x, offsets):
     return dy.new_empty(offsets.shape[0] - 1, dy.shape[1], x.shape[1])
 
 
+def _check_capture(t):
+    """A captured backward pass must not reach a node of the default stream (torch_binding.cpp)."""
+    if type(t) is torch.Tensor or type(t) is torch.nn.Parameter:
+        with torch.cuda.device(t.device):
+            ops._native().check_capture()
+
+
 def _grouped_setup(ctx, inputs, output):
     ctx.save_for_backward(*inputs)
 
 
 def _grouped_backward(ctx, dy):
     x, weight, offsets = ctx.saved_tensors
+    _check_capture(x)
     return (grouped_matmul_dgrad_op(dy, weight, offsets) if ctx.needs_input_grad[0] else None,
             grouped_matmul_wgrad_op(dy, x, offsets) if ctx.needs_input_grad[1] else None, None)
 
@@ -123,6 +131,7 @@ def _silu_setup(ctx, inputs, output):
 
 def _silu_backward(ctx, dy):
     gu, row_weight = ctx.saved_tensors
+    _check_capture(gu)
     dgu, dweight = silu_mul_backward_op(gu, dy, row_weight)
     return dgu, None if row_weight is None else dweight
 
