@@ -288,6 +288,18 @@ def test_every_kernel_of_the_product_is_reached():
     assert M.operator_status() == 0
 
 
+@pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
+@pytest.mark.parametrize("mnk", [(600, 7700, 7296), (7960, 3000, 2432), (2304, 18432, 1280)])
+def test_tiles_of_a_pair_of_ctas(mnk, quant):
+    """Sizes at which two CTAs share tiles of 256 x 256: a second half without rows, widths that are no
+    multiple of 8, odd numbers of K blocks, several bands of 2048 rows."""
+    m, n, k = mnk
+    a, sa, w, sw = block_inputs(m, n, k, quant, seed=m + n)
+    ref, mag = block_reference(a, sa, w, sw, quant)
+    close(M.matmul_block128(a, sa, w, sw, quant), ref, (k + 8) * U * mag)
+    assert M.operator_status() == 0
+
+
 # ----------------------------------------------------------------------------- the gated activation
 def silu_reference(gu, weight, dy):
     g, u = gu.double().chunk(2, 1)

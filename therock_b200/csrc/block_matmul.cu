@@ -20,19 +20,29 @@ CUresult byte_map(CUtensorMap* tm, const void* base, int64_t rows, int cols, int
   return encode_tensor_map(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
 }
 
-template <bool kHw>
-cudaError_t launch_tiles(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
-  static bool configured[kMaxDevices] = {false};
-  constexpr auto kernel = kHw ? fmoe_matmul_block128_hw_kernel : fmoe_matmul_block128_kernel;
-  constexpr int kSmem = kHw ? kHwSmemBytes : kBmmSmemBytes, kThreads = kHw ? kHwThreads : kBmmThreads;
+template <typename Kernel>
+cudaError_t launch_tiles(Kernel kernel, bool (&configured)[kMaxDevices], int threads, int smem, int cluster, const CUtensorMap& a,
+                         const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
   }
-  return launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmem, stream, a, w, p);
+  return launch_pdl_cluster(kernel, dim3(grid), dim3(threads), smem, cluster, stream, a, w, p);
+}
+template <bool kPair>
+cudaError_t launch_f32(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {false};
+  return launch_tiles(fmoe_matmul_block128_kernel<kPair>, configured, kBmmThreads, BmmCfg<kPair>::kSmemBytes, kPair ? 2 : 1, a, w, p,
+                      grid, stream);
+}
+template <bool kPair>
+cudaError_t launch_hw(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {false};
+  return launch_tiles(fmoe_matmul_block128_hw_kernel<kPair>, configured, kHwThreads, HwCfg<kPair>::kSmemBytes, kPair ? 2 : 1, a, w, p,
+                      grid, stream);
 }
 
 // Clusters of 1, 2, 4 and 8 CTAs that run side by side when a CTA has an SM to itself (a cluster does
@@ -118,25 +128,33 @@ int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p
   }
 }
 
-// Rows per tile of the kernel for few rows, 0 for the kernels with 128 x 256 tiles: whichever is
-// estimated to be done first.  An estimate is a fixed part (launch, set-up, the way of the first blocks,
-// the result) and a time for each K block of the longest CTA, in nanoseconds, fitted to measured times of
-// 1 to 2048 rows times weights of 1024 x 1024 up to 18432 x 7168; over those the choice is 1.1 % from
-// the best on average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times as many
-// at the same time; with 128 rows there are whole rounds.
-int small_rows(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
+// The kernel that is estimated to be done first: the one for few rows (16, 32 or 128 rows to a tile), or
+// 128 x 256 tiles of a CTA (kOneCta), or 256 x 256 tiles of a pair of CTAs (kPairOfCtas).  An estimate
+// is a fixed part (launch, set-up, the way of the first blocks, the result) and a time for each K block of
+// the longest CTA, in nanoseconds, fitted to measured times of 1 to 2048 rows times weights of 1024 x 1024
+// up to 18432 x 7168; over those the choice between few rows and 128 x 256 is 1.1 % from the best on
+// average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times as many at the same time;
+// with 128 rows there are whole rounds.  A pair starts 1.2 us later, but reads a third less from L2 and
+// shared memory, which under the power limit is a higher clock: 8192 x 4096 x 7168 takes 198 us instead of
+// 209 (power-of-two scales) and 241 instead of 253 (f32), 8192 x 1024 x 1024 12.2 instead of 11.6 and 16.1
+// instead of 14.8.
+enum : int { kOneCta = 0, kPairOfCtas = 1 };
+int choose_kernel(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
   const int64_t n_tiles = (n + 127) / 128;
   const int tile_n = hw ? kHwTileN : kBmmTileN;
-  const int64_t big_tiles = (m + kBmmTileM - 1) / kBmmTileM * ((n + tile_n - 1) / tile_n);
-  double best = (hw ? 4600.0 : 5000.0) + static_cast<double>((big_tiles + sms - 1) / sms) * kb * (hw ? 330.0 : 440.0);
-  int choice = 0;
+  const int64_t across = (n + tile_n - 1) / tile_n;
+  auto rounds_of = [](int64_t tiles, int64_t at_once) { return static_cast<double>((tiles + at_once - 1) / at_once); };
+  double best = (hw ? 4600.0 : 5000.0) + rounds_of((m + kBmmTileM - 1) / kBmmTileM * across, sms) * kb * (hw ? 330.0 : 440.0);
+  int choice = kOneCta;
+  const double pair = (hw ? 5700.0 : 6200.0) + rounds_of((m + 2 * kBmmTileM - 1) / (2 * kBmmTileM) * across, (sms + 1) / 2) * kb * (hw ? 305.0 : 418.0);
+  if (sms > 1 && pair < best) { best = pair; choice = kPairOfCtas; }
   const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2200, 300, 1.6}, {32, 3200, 360, 1.6}, {128, 6000, 420, 1.0}};
   for (const auto& kind : kinds) {
     const int64_t tiles = (m + kind.nt - 1) / kind.nt * n_tiles;
     if (tiles > (int64_t{1} << 20)) continue;
     const int split = 1 << small_log_split(kind.nt, static_cast<int>(tiles), kb, room);
     const int64_t ctas = tiles * split;
-    double rounds = kind.nt == 128 ? static_cast<double>((ctas + sms - 1) / sms) : static_cast<double>(ctas) / (sms * kind.shared);
+    double rounds = kind.nt == 128 ? rounds_of(ctas, sms) : static_cast<double>(ctas) / (sms * kind.shared);
     if (rounds < 1.0) rounds = 1.0;
     const double t = kind.fixed + (kb + split - 1) / split * kind.block * rounds;
     if (t < best) { best = t; choice = kind.nt; }
@@ -179,7 +197,8 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   const bool hw = quant == FMOE_QUANT_BLOCK128_UE8M0;
   ClusterRoom room;
   FMOE_CUDA((hw ? small_kernel_room<16, true>(&room) : small_kernel_room<16, false>(&room)));
-  if (const int nt = small_rows(m, n, k / 128, hw, sms, room)) {
+  const int choice = choose_kernel(m, n, k / 128, hw, sms, room);
+  if (choice != kOneCta && choice != kPairOfCtas) {
     BlockSmallParams p{};
     p.a_scale = a_scale;
     p.w_scale = w_scale;
@@ -188,12 +207,13 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
     p.kb = k / 128;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.status = status;
-    return hw ? run_small_nt<true>(nt, a, w, p, k, s) : run_small_nt<false>(nt, a, w, p, k, s);
+    return hw ? run_small_nt<true>(choice, a, w, p, k, s) : run_small_nt<false>(choice, a, w, p, k, s);
   }
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, m, k, kBmmTileM);
   const int tile_n = hw ? kHwTileN : kBmmTileN;
-  if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, tile_n);
+  const bool pair = choice == kPairOfCtas;
+  if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, !pair ? tile_n : hw ? HwCfg<true>::kWRows : BmmCfg<true>::kHalfRows);
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
   BlockMatmulParams p{};
   p.a_scale = a_scale;
@@ -201,14 +221,20 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   p.m = static_cast<int>(m);
   p.n = n;
   p.kb = k / 128;
-  p.m_blocks = (p.m + kBmmTileM - 1) / kBmmTileM;
+  const int tile_m = pair ? 2 * kBmmTileM : kBmmTileM;
+  p.m_blocks = (p.m + tile_m - 1) / tile_m;
   p.n_blocks = (n + tile_n - 1) / tile_n;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.idesc = hw ? ptx::make_idesc_block_scaled(kBmmTileM, kHwTileN) : ptx::make_idesc(0u, kBmmTileM, kBmmTileN / 2);
+  p.idesc = hw ? ptx::make_idesc_block_scaled(tile_m, kHwTileN) : ptx::make_idesc(0u, tile_m, kBmmTileN / 2);
   const int tiles = p.m_blocks * p.n_blocks;
-  const int grid = tiles < sms ? tiles : sms;
-  FMOE_CUDA(hw ? launch_tiles<true>(ta, tw, p, grid, s) : launch_tiles<false>(ta, tw, p, grid, s));
+  if (pair) {
+    const int grid = 2 * (tiles < sms / 2 ? tiles : sms / 2);      // sms / 2 pairs run at once, or take turns: none waits for another
+    FMOE_CUDA(hw ? launch_hw<true>(ta, tw, p, grid, s) : launch_f32<true>(ta, tw, p, grid, s));
+  } else {
+    const int grid = tiles < sms ? tiles : sms;
+    FMOE_CUDA(hw ? launch_hw<false>(ta, tw, p, grid, s) : launch_f32<false>(ta, tw, p, grid, s));
+  }
   return FMOE_OK;
 }
 

@@ -14,10 +14,15 @@
 // of the stage), and the epilogue's loop takes four K blocks at a time with all addresses and parities in
 // registers.
 //
-// Measured on a B200, 8192 x 4096 x 7168: 219 us = 2193 TFLOP/s, 770 cycles a stage at the 1.6 GHz that the
-// power limit leaves; a library e4m3 product without block scales sustains 2606 there.  One issuing warp
-// and one 256-column accumulator per stage took 245 us, sixteen epilogue warps of 64 columns 272, and
-// 192-column tiles whose accumulator is read at once 246.
+// Large products are also bound by power.  There two CTAs share a tile of 256 rows (kPair): each holds its
+// own 128 activation rows and half of the weight rows, so that a third less comes from L2 and the MMAs
+// read a third less of shared memory, and the tiles go through the result in bands.
+//
+// Measured on a B200, 8192 x 4096 x 7168: 201 us = 2393 TFLOP/s in a short run; back to back under the power
+// limit 241 us = 1996 TFLOP/s at 1420 MHz (one CTA to a tile: 212 and 253 at 1360 MHz; without bands 219 and
+// 260).  A library e4m3 product without block scales takes 195 us back to back.  In a short run and without
+// bands one issuing warp and one 256-column accumulator per stage took 245 us, sixteen epilogue warps of 64
+// columns 272, and 192-column tiles whose accumulator is read at once 246.
 //
 // A separate warp loads the scales of four blocks at a time, multiplies the activations' by those of the
 // tile's two weight blocks and leaves the products in shared memory.
@@ -32,17 +37,21 @@ namespace fmoe {
 
 constexpr int kBmmThreads = 512;          // warps 0, 1: TMA, scales; 4-7: MMA; 8-15: epilogue
 constexpr int kBmmEpiWarps = 8;
-constexpr int kBmmStages = 4;
 constexpr int kBmmTileM = 128, kBmmTileN = 256;
 constexpr int kBmmABytes = kBmmTileM * 128;
-constexpr int kBmmStageBytes = kBmmABytes + kBmmTileN * 128;
 constexpr int kBmmScaleSlots = 2;         // ring of scale products, four K blocks a slot
 constexpr int kBmmScaleSlotFloats = 4 * 2 * kBmmTileM;
 constexpr int kBmmEpiPitch = 8;           // words: 16 bf16 columns of a row
 constexpr int kBmmEpiBytes = kBmmEpiWarps * 32 * kBmmEpiPitch * 4;
 constexpr int kBmmMisc = 256;
-constexpr int kBmmSmemBytes = kBmmStages * kBmmStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
-static_assert(kBmmSmemBytes <= 227 * 1024, "shared memory budget");
+template <bool kPair> struct BmmCfg {
+  static constexpr int kHalfRows = kPair ? 64 : 128;        // weight rows of half a tile in a CTA's shared memory
+  static constexpr int kStageBytes = kBmmABytes + 2 * kHalfRows * 128;
+  static constexpr int kTileM = kPair ? 2 * kBmmTileM : kBmmTileM;
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
+  static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA to an SM: each takes all of its tensor memory");
+};
 // setmaxnreg redistributes the 512 x 128 registers of the launch: what the roles take must not exceed it.
 constexpr int kBmmThinRegs = 80, kBmmIssueRegs = 40, kBmmFatRegs = 184;
 static_assert(128 * (kBmmThinRegs + kBmmIssueRegs) + 256 * kBmmFatRegs <= kBmmThreads * 128, "register budget");
@@ -58,6 +67,19 @@ struct BlockMatmulParams {
   int* status;              // may be null
   uint32_t idesc;
 };
+
+// Tile order: bands of 2048 rows, in a band column by column.  The tiles that run side by side are then
+// about as high as wide, and read half of what a single band of 8192 rows made them read.
+struct BlockTile {
+  int m, n;                 // in tiles
+};
+template <int kTileM>
+__device__ __forceinline__ BlockTile decode_block_tile(int tile, int m_blocks, int n_blocks) {
+  constexpr int kBand = 2048 / kTileM;
+  const int band = tile / (kBand * n_blocks), local = tile - band * (kBand * n_blocks);
+  const int height = min(kBand, m_blocks - band * kBand), n = local / height;
+  return {band * kBand + local - n * height, n};
+}
 
 static __device__ int g_bmm_status;      // for calls without a status word
 
@@ -110,9 +132,12 @@ __device__ __forceinline__ void store_rows_bf16(const float (&acc)[kCols], uint3
   }
 }
 
+template <bool kPair>
 __global__ void __launch_bounds__(kBmmThreads, 1)
 fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                             const BlockMatmulParams p) {
+  using Cfg = BmmCfg<kPair>;
+  constexpr int kBmmStages = Cfg::kStages, kBmmStageBytes = Cfg::kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* misc = smem + kBmmStages * kBmmStageBytes;
@@ -129,6 +154,8 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
 
   const int warp = ptx::warp_index();
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? ptx::cluster_ctarank() : 0u;
+  const int first_tile = kPair ? blockIdx.x >> 1 : blockIdx.x, tile_step = kPair ? gridDim.x >> 1 : gridDim.x;
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_a);
     ptx::prefetch_tensormap(&tm_w);
@@ -138,7 +165,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     }
     for (int b = 0; b < 4; ++b) {
       ptx::mbar_init(ptx::smem_u32(&part_full_bar[b]), 1);
-      ptx::mbar_init(ptx::smem_u32(&part_empty_bar[b]), kBmmEpiWarps / 2);
+      ptx::mbar_init(ptx::smem_u32(&part_empty_bar[b]), kPair ? kBmmEpiWarps : kBmmEpiWarps / 2);
     }
     for (int i = 0; i < kBmmScaleSlots; ++i) {
       ptx::mbar_init(ptx::smem_u32(&sc_full_bar[i]), 32);
@@ -149,12 +176,18 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     ptx::fence_proxy_async();
   }
   if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
-    ptx::tmem_relinquish();
+    if (kPair) {
+      ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::pdl_wait();
   ptx::tc_fence_before();
-  __syncthreads();
+  if (kPair) ptx::cluster_sync_all();      // both CTAs' barriers are initialised before anyone signals them
+  else __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = p.m_blocks * p.n_blocks;
@@ -163,19 +196,29 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     ptx::setmaxnreg_dec<kBmmThinRegs>();
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer
-      const uint32_t full0 = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar), smem0 = ptx::smem_u32(smem);
+      const uint32_t full_own = ptx::smem_u32(full_bar), empty0 = ptx::smem_u32(empty_bar), smem0 = ptx::smem_u32(smem);
+      const uint32_t full0 = kPair ? ptx::map_to_rank(full_own, 0) : full_own;      // both CTAs' bytes go to rank 0
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-        const int m0 = tile % p.m_blocks * kBmmTileM, n0 = tile / p.m_blocks * kBmmTileN;
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        const BlockTile at = decode_block_tile<kBmmTileM>(tile, p.m_blocks, p.n_blocks);
+        const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM;
+        const int n0 = at.n * kBmmTileN + static_cast<int>(rank) * Cfg::kHalfRows;
         for (int k = 0; k < p.kb; ++k) {
           if (!ptx::mbar_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag)) { ok = false; break; }
           if (ptx::elect_one()) {
             const uint32_t full = full0 + 8 * stage, sa = smem0 + stage * kBmmStageBytes;
-            ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
-            ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
-            ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+            if (kPair) {
+              if (rank == 0) ptx::mbar_arrive_expect_tx(full_own + 8 * stage, 2 * kBmmStageBytes);
+              ptx::tma_load_2d_pair(sa, &tm_a, full, k * 128, m0);
+              ptx::tma_load_2d_pair(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+              ptx::tma_load_2d_pair(sa + kBmmABytes + Cfg::kHalfRows * 128, &tm_w, full, k * 128, n0 + 128);
+            } else {
+              ptx::mbar_arrive_expect_tx(full, kBmmStageBytes);
+              ptx::tma_load_2d(sa, &tm_a, full, k * 128, m0);
+              ptx::tma_load_2d(sa + kBmmABytes, &tm_w, full, k * 128, n0);
+            }
           }
           __syncwarp();
           if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
@@ -190,8 +233,9 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       bool ok = true;
       const int nb = (p.n + 127) >> 7;
       const bool vec = (p.kb & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-        const int m0 = tile % p.m_blocks * kBmmTileM, nb0 = tile / p.m_blocks * 2;
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        const BlockTile at = decode_block_tile<kBmmTileM>(tile, p.m_blocks, p.n_blocks);
+        const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM, nb0 = at.n * 2;
         const float* sw0 = p.w_scale + static_cast<size_t>(nb0) * p.kb;
         const float* sw1 = p.w_scale + static_cast<size_t>(min(nb0 + 1, nb - 1)) * p.kb;
         for (int k = 0; k < p.kb; k += 4) {
@@ -238,30 +282,42 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     ptx::setmaxnreg_dec<kBmmIssueRegs>();
     // ------------------------------------------------------------------ MMA issuers
     const int half = (warp >> 1) & 1, parity = warp & 1;
-    static_assert(kBmmStages == 4, "an issuer goes to and fro between two stages");
+    static_assert(kBmmStages % 2 == 0, "an issuer has the stages of its parity");
     const uint32_t full0 = ptx::smem_u32(full_bar) + 8 * parity, empty0 = ptx::smem_u32(empty_bar) + 8 * parity;
     const uint32_t part_full = ptx::smem_u32(part_full_bar) + 8 * (2 * half + parity), part_empty = ptx::smem_u32(part_empty_bar) + 8 * (2 * half + parity);
     constexpr uint64_t kDesc = ptx::sw128_kmajor_desc_template();
     const uint32_t smem0 = ptx::smem_u32(smem) + parity * kBmmStageBytes;
     const uint64_t da0 = ptx::make_smem_desc(kDesc, smem0);
-    const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kBmmABytes + half * 128 * 128);
+    const uint64_t db0 = ptx::make_smem_desc(kDesc, smem0 + kBmmABytes + half * Cfg::kHalfRows * 128);
     const uint32_t d_tmem = tmem_base + half * 256 + parity * 128;
-    const int my_tiles = blockIdx.x < total_tiles ? (total_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+    const int my_tiles = rank == 0 && first_tile < total_tiles ? (total_tiles - 1 - first_tile) / tile_step + 1 : 0;
+    const uint32_t part_full_peer = kPair ? ptx::map_to_rank(part_full, 1) : 0u, empty_peer = kPair ? ptx::map_to_rank(empty0, 1) : 0u;
     const long long stages = static_cast<long long>(my_tiles) * p.kb;
-    uint32_t phase = 0;
+    uint32_t phase = 0, part_phase = 1;
     bool ok = true;
-    for (long long it = parity; ok && it < stages; it += 4) {
+    for (long long it = parity; ok && it < stages; it += kBmmStages) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {             // stages parity and parity + 2
+      for (int h = 0; h < kBmmStages / 2; ++h) {             // stages parity, parity + 2, ...
         if (it + 2 * h >= stages) break;
-        if (!ptx::mbar_wait(full0 + 16 * h, phase, abort_flag) || !ptx::mbar_wait(part_empty, h ^ 1u, abort_flag)) { ok = false; break; }
+        if (!ptx::mbar_wait(full0 + 16 * h, phase, abort_flag) || !ptx::mbar_wait(part_empty, part_phase, abort_flag)) { ok = false; break; }
+        part_phase ^= 1u;
         ptx::tc_fence_after();
         if (ptx::elect_one()) {
           constexpr uint32_t kTwo = (2 * kBmmStageBytes) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) ptx::umma_f8(d_tmem, da0 + (h * kTwo + kk * 2), db0 + (h * kTwo + kk * 2), p.idesc, kk ? 1u : 0u);
-          ptx::umma_commit(part_full);
-          ptx::umma_commit(empty0 + 16 * h);
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kPair) ptx::umma_f8_pair(d_tmem, da0 + (h * kTwo + kk * 2), db0 + (h * kTwo + kk * 2), p.idesc, kk ? 1u : 0u);
+            else ptx::umma_f8(d_tmem, da0 + (h * kTwo + kk * 2), db0 + (h * kTwo + kk * 2), p.idesc, kk ? 1u : 0u);
+          }
+          if (kPair) {      // in both CTAs
+            ptx::umma_commit_pair(part_full);
+            ptx::umma_commit_pair(part_full_peer);
+            ptx::umma_commit_pair(empty0 + 16 * h);
+            ptx::umma_commit_pair(empty_peer + 16 * h);
+          } else {
+            ptx::umma_commit(part_full);
+            ptx::umma_commit(empty0 + 16 * h);
+          }
         }
         __syncwarp();
       }
@@ -275,7 +331,8 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     const int half = (warp - 8) >> 2;
     uint32_t* mine = epi + (warp - 8) * (32 * kBmmEpiPitch);
     // x is the accumulator that the first and the third of four K blocks are in, y the other one.
-    const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty0 = ptx::smem_u32(part_empty_bar) + 16 * half;
+    const uint32_t part_full0 = ptx::smem_u32(part_full_bar) + 16 * half, part_empty_own = ptx::smem_u32(part_empty_bar) + 16 * half;
+    const uint32_t part_empty0 = kPair ? ptx::map_to_rank(part_empty_own, 0) : part_empty_own;      // the issuers are in rank 0
     uint32_t full_x = part_full0, full_y = part_full0 + 8, empty_x = part_empty0, empty_y = part_empty0 + 8;
     uint32_t t_x = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * 256), t_y = t_x + 128;
     uint32_t phase_x = 0, phase_y = 0;
@@ -284,12 +341,13 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     uint32_t sc_empty_now = ptx::smem_u32(sc_empty_bar), sc_empty_next = sc_empty_now + 8;
     int slot_now = 0, slot_next = kBmmScaleSlotFloats;
     uint32_t sc_phase = 0;                               // of both slots: flips every two groups
-    const int kb = p.kb, m_blocks = p.m_blocks;
+    const int kb = p.kb, m_blocks = p.m_blocks, n_blocks = p.n_blocks;
     const bool leader = lane == 0;
     const float* sc_base = sc_ring + half * kBmmTileM + quad * 32 + lane;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-      const int m0 = tile % m_blocks * kBmmTileM, n0 = tile / m_blocks * kBmmTileN;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      const BlockTile at = decode_block_tile<kBmmTileM>(tile, m_blocks, n_blocks);
+      const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM, n0 = at.n * kBmmTileN;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
@@ -320,7 +378,8 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
               ptx::tmem_ld_wait();
               if (c == 3) {      // everything has left this accumulator: the MMAs may overwrite it
                 ptx::tc_fence_before();
-                ptx::mbar_arrive_if((u & 1) ? empty_y : empty_x, leader);
+                if (kPair) ptx::mbar_arrive_cluster_relaxed_if((u & 1) ? empty_y : empty_x, leader);
+                else ptx::mbar_arrive_if((u & 1) ? empty_y : empty_x, leader);
                 if (u & 1) phase_y ^= 1u; else phase_x ^= 1u;
               }
 #pragma unroll
@@ -344,10 +403,12 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
   }
 
   ptx::tc_fence_before();
-  __syncthreads();
+  if (kPair) ptx::cluster_sync_all();      // neither CTA leaves while its partner can still signal it or read its shared memory
+  else __syncthreads();
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem_base, 512);
+    if (kPair) ptx::tmem_dealloc_pair(tmem_base, 512);
+    else ptx::tmem_dealloc(tmem_base, 512);
   }
 }
 
