@@ -292,7 +292,7 @@ def test_every_kernel_of_the_product_is_reached():
 @pytest.mark.parametrize("mnk", [(600, 7700, 7296), (7960, 3000, 2432), (2304, 18432, 1280)])
 def test_tiles_of_a_pair_of_ctas(mnk, quant):
     """Sizes at which two CTAs share tiles of 256 x 256: a second half without rows, widths that are no
-    multiple of 8, odd numbers of K blocks, several bands of 2048 rows."""
+    multiple of 8, odd numbers of K blocks, several bands of rows."""
     m, n, k = mnk
     a, sa, w, sw = block_inputs(m, n, k, quant, seed=m + n)
     ref, mag = block_reference(a, sa, w, sw, quant)

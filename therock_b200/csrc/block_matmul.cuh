@@ -48,7 +48,7 @@ template <bool kPair> struct BmmCfg {
   static constexpr int kHalfRows = kPair ? 64 : 128;        // weight rows of half a tile in a CTA's shared memory
   static constexpr int kStageBytes = kBmmABytes + 2 * kHalfRows * 128;
   static constexpr int kTileM = kPair ? 2 * kBmmTileM : kBmmTileM;
-  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStages = 4;                         // six for a pair cost 1.3 % (8192 x 4096 x 7168)
   static constexpr int kSmemBytes = kStages * kStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
   static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA to an SM: each takes all of its tensor memory");
 };
@@ -68,14 +68,15 @@ struct BlockMatmulParams {
   uint32_t idesc;
 };
 
-// Tile order: bands of 2048 rows, in a band column by column.  The tiles that run side by side are then
-// about as high as wide, and read half of what a single band of 8192 rows made them read.
+// Tile order: bands of 1024 rows, in a band column by column.  The tiles that run side by side then read
+// 1024 rows and a few thousand columns, half of what a single band of 8192 rows made them read (and 218 ->
+// 210 us for 8192 x 4096 x 7168 with power-of-two scales; bands of 2048 and 4096 rows are as good).
 struct BlockTile {
   int m, n;                 // in tiles
 };
 template <int kTileM>
 __device__ __forceinline__ BlockTile decode_block_tile(int tile, int m_blocks, int n_blocks) {
-  constexpr int kBand = 2048 / kTileM;
+  constexpr int kBand = 1024 / kTileM;
   const int band = tile / (kBand * n_blocks), local = tile - band * (kBand * n_blocks);
   const int height = min(kBand, m_blocks - band * kBand), n = local / height;
   return {band * kBand + local - n * height, n};
@@ -202,7 +203,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
-        const BlockTile at = decode_block_tile<kBmmTileM>(tile, p.m_blocks, p.n_blocks);
+        const BlockTile at = decode_block_tile<Cfg::kTileM>(tile, p.m_blocks, p.n_blocks);
         const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM;
         const int n0 = at.n * kBmmTileN + static_cast<int>(rank) * Cfg::kHalfRows;
         for (int k = 0; k < p.kb; ++k) {
@@ -234,7 +235,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       const int nb = (p.n + 127) >> 7;
       const bool vec = (p.kb & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 15) == 0;
       for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
-        const BlockTile at = decode_block_tile<kBmmTileM>(tile, p.m_blocks, p.n_blocks);
+        const BlockTile at = decode_block_tile<Cfg::kTileM>(tile, p.m_blocks, p.n_blocks);
         const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM, nb0 = at.n * 2;
         const float* sw0 = p.w_scale + static_cast<size_t>(nb0) * p.kb;
         const float* sw1 = p.w_scale + static_cast<size_t>(min(nb0 + 1, nb - 1)) * p.kb;
@@ -346,7 +347,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     const float* sc_base = sc_ring + half * kBmmTileM + quad * 32 + lane;
     bool ok = true;
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
-      const BlockTile at = decode_block_tile<kBmmTileM>(tile, m_blocks, n_blocks);
+      const BlockTile at = decode_block_tile<Cfg::kTileM>(tile, m_blocks, n_blocks);
       const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM, n0 = at.n * kBmmTileN;
       float acc[128];
 #pragma unroll
