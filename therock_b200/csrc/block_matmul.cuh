@@ -19,7 +19,7 @@
 // read a third less of shared memory, and the tiles go through the result in bands.
 //
 // Measured on a B200, 8192 x 4096 x 7168: 201 us = 2393 TFLOP/s in a short run; back to back under the power
-// limit 241 us = 1996 TFLOP/s at 1420 MHz (one CTA to a tile: 212 and 253 at 1360 MHz; without bands 219 and
+// limit 237 us = 2030 TFLOP/s at 1410 MHz (one CTA to a tile: 212 and 253 at 1360 MHz; without bands 219 and
 // 260).  A library e4m3 product without block scales takes 195 us back to back.  In a short run and without
 // bands one issuing warp and one 256-column accumulator per stage took 245 us, sixteen epilogue warps of 64
 // columns 272, and 192-column tiles whose accumulator is read at once 246.
