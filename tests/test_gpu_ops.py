@@ -289,6 +289,20 @@ def test_every_kernel_of_the_product_is_reached():
 
 
 @pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
+@pytest.mark.parametrize("mnk", [(5, 63, 128), (5, 63, 640), (5, 63, 1024), (5, 63, 2048), (250, 4999, 384), (639, 200, 1408), (640, 63, 4096),
+                                 (300, 63, 7168), (100, 18431, 640), (130, 2303, 5632), (130, 1100, 7168), (639, 200, 5632),
+                                 (1030, 7743, 128), (333, 18431, 128), (2040, 2300, 3968)])
+def test_every_form_of_the_choice(mnk, quant):
+    """Sizes for 16, 32 and 128 rows to a tile, each with K whole and shared by 2, 4 and 8 CTAs, and for
+    128 x 256 tiles of one CTA, by the estimates that choose among them."""
+    m, n, k = mnk
+    a, sa, w, sw = block_inputs(m, n, k, quant, seed=m + n)
+    ref, mag = block_reference(a, sa, w, sw, quant)
+    close(M.matmul_block128(a, sa, w, sw, quant), ref, (k + 8) * U * mag)
+    assert M.operator_status() == 0
+
+
+@pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
 @pytest.mark.parametrize("mnk", [(600, 7700, 7296), (7960, 3000, 2432), (2304, 18432, 1280)])
 def test_tiles_of_a_pair_of_ctas(mnk, quant):
     """Sizes at which two CTAs share tiles of 256 x 256: a second half without rows, widths that are no

@@ -130,8 +130,8 @@ int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p
 
 // The kernel that is estimated to be done first: the one for few rows (16, 32 or 128 rows to a tile), or
 // 128 x 256 tiles of a CTA (kOneCta), or 256 x 256 tiles of a pair of CTAs (kPairOfCtas).  An estimate
-// is a fixed part (launch, set-up, the way of the first blocks, the result) and a time for each K block of
-// the longest CTA, in nanoseconds, fitted to measured times of 1 to 2048 rows times weights of 1024 x 1024
+// is a fixed part (launch, set-up, the way of the first blocks, the result), with few rows one for each
+// halving of K over a cluster, and a time for each K block of the longest CTA, in nanoseconds, fitted to measured times of 1 to 2048 rows times weights of 1024 x 1024
 // up to 18432 x 7168; over those the choice between few rows and 128 x 256 is 1.1 % from the best on
 // average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times as many at the same time;
 // with 128 rows there are whole rounds.  A pair starts 1.2 us later, but reads a third less from L2 and
@@ -148,15 +148,16 @@ int choose_kernel(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom&
   int choice = kOneCta;
   const double pair = (hw ? 5700.0 : 6200.0) + rounds_of((m + 2 * kBmmTileM - 1) / (2 * kBmmTileM) * across, (sms + 1) / 2) * kb * (hw ? 305.0 : 418.0);
   if (sms > 1 && pair < best) { best = pair; choice = kPairOfCtas; }
-  const struct { int nt; double fixed, block, shared; } kinds[3] = {{16, 2200, 300, 1.6}, {32, 3200, 360, 1.6}, {128, 6000, 420, 1.0}};
+  const struct { int nt; double fixed, halving, block, shared; } kinds[3] = {
+      {16, 2000, 100, 300, 1.6}, {32, 3000, 200, 345, 1.6}, {128, 4800, 1200, 380, 1.0}};
   for (const auto& kind : kinds) {
     const int64_t tiles = (m + kind.nt - 1) / kind.nt * n_tiles;
     if (tiles > (int64_t{1} << 20)) continue;
-    const int split = 1 << small_log_split(kind.nt, static_cast<int>(tiles), kb, room);
+    const int log_split = small_log_split(kind.nt, static_cast<int>(tiles), kb, room), split = 1 << log_split;
     const int64_t ctas = tiles * split;
     double rounds = kind.nt == 128 ? rounds_of(ctas, sms) : static_cast<double>(ctas) / (sms * kind.shared);
     if (rounds < 1.0) rounds = 1.0;
-    const double t = kind.fixed + (kb + split - 1) / split * kind.block * rounds;
+    const double t = kind.fixed + log_split * kind.halving + (kb + split - 1) / split * kind.block * rounds;
     if (t < best) { best = t; choice = kind.nt; }
   }
   return choice;

@@ -49,8 +49,12 @@ template <bool kPair> struct BmmCfg {
   static constexpr int kStageBytes = kBmmABytes + 2 * kHalfRows * 128;
   static constexpr int kTileM = kPair ? 2 * kBmmTileM : kBmmTileM;
   static constexpr int kStages = 4;                         // six for a pair cost 1.3 % (8192 x 4096 x 7168)
-  static constexpr int kSmemBytes = kStages * kStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
-  static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA to an SM: each takes all of its tensor memory");
+  static constexpr int kUsedBytes = kStages * kStageBytes + kBmmMisc + kBmmScaleSlots * kBmmScaleSlotFloats * 4 + kBmmEpiBytes + 1024;
+  // A CTA takes all of its SM's tensor memory, and a pair holds one SM's while it waits for the other's.
+  // With this much shared memory nothing that uses tensor memory is on an SM at the same time (a cluster
+  // of the kernel for few rows, on another stream, could hold the one and wait for the other).
+  static constexpr int kSmemBytes = kUsedBytes < 184 * 1024 ? 184 * 1024 : kUsedBytes;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 // setmaxnreg redistributes the 512 x 128 registers of the launch: what the roles take must not exceed it.
 constexpr int kBmmThinRegs = 80, kBmmIssueRegs = 40, kBmmFatRegs = 184;

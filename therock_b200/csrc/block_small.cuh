@@ -43,6 +43,7 @@ template <int kNT> struct BlockSmallCfg {
   static constexpr int kMinSmem = (kTmemCols == 128 ? 56 : kTmemCols == 256 ? 113 : 200) * 1024;
   static constexpr int kStageBytes = kBsWBytes + kNT * 128;
   static constexpr int kScaleBytes = kBsScaleSlots * 4 * kNT * 4;
+  static_assert(184 * 1024 + kMinSmem > 227 * 1024, "not beside a CTA of a pair (see BmmCfg)");
   static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "see kMinSmem");
   static constexpr int smem_bytes(int stages, bool split) {
     return stages * kStageBytes + kBsMisc + kScaleBytes + (split ? kNT * 128 * 4 : 0) + 1024;
