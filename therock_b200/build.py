@@ -30,14 +30,18 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
-def build(force: bool = False, verbose: bool = False, checked: bool = False, timing_switches: bool = False) -> str:
+def build(force: bool = False, verbose: bool = False, checked: bool = False, timing_switches: bool = False,
+          wait_limit_switch: bool = False) -> str:
     """Builds the product library, or with checked=True libfmoe_b200_checked.so (the same
     sources with -DFMOE_BOUNDS_CHECKS), or with timing_switches=True libfmoe_b200_timing.so
     (-DFMOE_TIMING_SWITCHES: FMOE_DEBUG_FLAGS / FMOE_GEMM_MODE are honoured; results are invalid
-    while they are set).  The variants never replace the product library."""
-    if checked or timing_switches:
-        return _build_variant("checked" if checked else "timing",
-                              ["-DFMOE_BOUNDS_CHECKS"] if checked else ["-DFMOE_TIMING_SWITCHES"], force, verbose)
+    while they are set), or with wait_limit_switch=True libfmoe_b200_waits.so (-DFMOE_WAIT_LIMIT_SWITCH:
+    fmoe_set_wait_limit sets how long a wait in a kernel may take).  The variants never replace the
+    product library."""
+    for on, suffix, define in ((checked, "checked", "-DFMOE_BOUNDS_CHECKS"), (timing_switches, "timing", "-DFMOE_TIMING_SWITCHES"),
+                               (wait_limit_switch, "waits", "-DFMOE_WAIT_LIMIT_SWITCH")):
+        if on:
+            return _build_variant(suffix, [define], force, verbose)
     lib = _build_variant("", [], force, verbose)
     build_binding(force, verbose)
     return lib

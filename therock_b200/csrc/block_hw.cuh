@@ -129,7 +129,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
         if (++stage == kHwStages) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x21);
+    if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x21);
     ptx::pdl_release();
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------------ MMA issuer: four K blocks at a time
@@ -200,7 +200,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
       if (ptx::elect_one()) commit(acc_full, kPair ? ptx::map_to_rank(acc_full, 1) : 0u);
       __syncwarp();
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x22);
+    if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x22);
   } else if (warp == 2 || warp == 3) {
     // ------------------------------------------------------------------ scale images
     // Two warps take the groups of four K blocks in turn: one alone, with a load's latency and an arrival
@@ -250,7 +250,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
         slot ^= 2;
       }
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x23);
+    if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x23);
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ drain and epilogue
     const uint32_t acc_full = ptx::smem_u32(acc_full_bar), acc_empty_own = ptx::smem_u32(acc_empty_bar);
@@ -282,12 +282,14 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
       for (int j = 0; j < 128; ++j) acc[j] = __uint_as_float(v[j >> 5][j & 31]);
       store_rows_bf16<128>(acc, mine, p.out, m0 + quad * 32, p.m, n0 + half * 128, p.n);
     }
-    if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x24);
+    if (!ok && threadIdx.x == 128) bmm_fail<kPair>(p.status, abort_flag, 0x24);
   }
 
+  __syncwarp();
   ptx::tc_fence_before();
   if (kPair) ptx::cluster_sync_all();      // neither CTA leaves while its partner can still signal it or read its shared memory
   else __syncthreads();
+  ptx::settle(abort_flag);
   if (warp == 1) {
     ptx::tc_fence_after();
     if (kPair) ptx::tmem_dealloc_pair(tmem_base, 512);

@@ -171,6 +171,12 @@ cudaError_t take_block_matmul_status(int32_t* code) {
   if (e == cudaSuccess && *code != 0) e = cudaMemcpyToSymbol(g_bmm_status, &zero, sizeof(zero));
   return e;
 }
+#ifdef FMOE_WAIT_LIMIT_SWITCH
+cudaError_t set_block_matmul_wait_limit(int64_t cycles) {
+  const long long limit = cycles;
+  return cudaMemcpyToSymbol(ptx::g_wait_limit, &limit, sizeof(limit));
+}
+#endif
 }  // namespace fmoe
 
 extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
@@ -255,3 +261,14 @@ extern "C" int fmoe_operator_status(int32_t device, int32_t* status_out) {
   *status_out = code[0] ? code[0] : code[1];
   return FMOE_OK;
 }
+
+#ifdef FMOE_WAIT_LIMIT_SWITCH
+// Limit of one wait in the operators' kernels, in clock cycles, on the current device.
+extern "C" FMOE_API int fmoe_set_wait_limit(int64_t cycles) {
+  using namespace fmoe;
+  FMOE_CUDA(cudaDeviceSynchronize());
+  FMOE_CUDA(set_grouped_wait_limit(cycles));
+  FMOE_CUDA(set_block_matmul_wait_limit(cycles));
+  return FMOE_OK;
+}
+#endif

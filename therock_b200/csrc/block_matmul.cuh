@@ -88,8 +88,11 @@ __device__ __forceinline__ BlockTile decode_block_tile(int tile, int m_blocks, i
 
 static __device__ int g_bmm_status;      // for calls without a status word
 
-__device__ __forceinline__ void bmm_fail(int* status, int code) {
+// kPair: both CTAs of a pair give up.
+template <bool kPair>
+__device__ __forceinline__ void bmm_fail(int* status, volatile int* abort_flag, int code) {
   atomicExch(status != nullptr ? status : &g_bmm_status, kStatusBmmTimeout | code);
+  if (kPair) ptx::raise_in_peer(abort_flag);
 }
 
 // Exponent byte -> power of two (0 is 2^-127, 255 is NaN).
@@ -229,7 +232,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
           if (++stage == kBmmStages) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok && lane == 0) bmm_fail(p.status, 0x01);
+      if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x01);
       ptx::pdl_release();
     } else if (warp == 1) {
       // ---------------------------------------------------------------- scale products
@@ -281,7 +284,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
           if (++slot == kBmmScaleSlots) { slot = 0; sphase ^= 1u; }
         }
       }
-      if (!ok && lane == 0) bmm_fail(p.status, 0x03);
+      if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x03);
     }
   } else if (warp < 8) {
     ptx::setmaxnreg_dec<kBmmIssueRegs>();
@@ -328,7 +331,7 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       }
       phase ^= 1u;
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x02);
+    if (!ok && lane == 0) bmm_fail<kPair>(p.status, abort_flag, 0x02);
   } else {
     // ------------------------------------------------------------------ promotion and epilogue
     ptx::setmaxnreg_inc<kBmmFatRegs>();
@@ -404,12 +407,14 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
       if (!ok) break;
       store_rows_bf16<128>(acc, mine, p.out, m0 + quad * 32, p.m, n0 + half * 128, p.n);
     }
-    if (!ok && threadIdx.x == 256) bmm_fail(p.status, 0x04);
+    if (!ok && threadIdx.x == 256) bmm_fail<kPair>(p.status, abort_flag, 0x04);
   }
 
+  __syncwarp();
   ptx::tc_fence_before();
   if (kPair) ptx::cluster_sync_all();      // neither CTA leaves while its partner can still signal it or read its shared memory
   else __syncthreads();
+  ptx::settle(abort_flag);
   if (warp == 1) {
     ptx::tc_fence_after();
     if (kPair) ptx::tmem_dealloc_pair(tmem_base, 512);

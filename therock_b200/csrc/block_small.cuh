@@ -136,7 +136,7 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       __syncwarp();
       if (++stage == p.stages) { stage = 0; phase ^= 1u; }
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x11);
+    if (!ok && lane == 0) bmm_fail<false>(p.status, abort_flag, 0x11);
     ptx::pdl_release();
   } else if (warp & 1 && warp < 4) {
     // ------------------------------------------------------------------ MMA issuers
@@ -174,7 +174,7 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       }
       buf_phase ^= 1u;
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x12);
+    if (!ok && lane == 0) bmm_fail<false>(p.status, abort_flag, 0x12);
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scale products
     // The next slot is requested before the present one is handed over: two slots, eight blocks of K, are
@@ -243,7 +243,7 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       request(k + 8, s[0], w[0]);
       hand_over(k + 4, s[1], w[1]);
     }
-    if (!ok && lane == 0) bmm_fail(p.status, 0x13);
+    if (!ok && lane == 0) bmm_fail<false>(p.status, abort_flag, 0x13);
   }
 
   float acc[Cfg::kCols];
@@ -298,7 +298,7 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
       __syncwarp();
       ptx::mbar_arrive_if(sc_empty0 + 8 * slot, lane == 0);
     }
-    if (!ok && threadIdx.x == 128) bmm_fail(p.status, 0x14);
+    if (!ok && threadIdx.x == 128) bmm_fail<false>(p.status, abort_flag, 0x14);
   }
 
   const int out_col = n_blk * 128 + row;
@@ -344,8 +344,10 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     }
   }
 
+  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
+  ptx::settle(abort_flag);
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);

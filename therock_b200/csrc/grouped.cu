@@ -86,6 +86,12 @@ cudaError_t take_grouped_status(int32_t* code) {
   if (e == cudaSuccess && *code != 0) e = cudaMemcpyToSymbol(g_grouped_status, &zero, sizeof(zero));
   return e;
 }
+#ifdef FMOE_WAIT_LIMIT_SWITCH
+cudaError_t set_grouped_wait_limit(int64_t cycles) {
+  const long long limit = cycles;
+  return cudaMemcpyToSymbol(ptx::g_wait_limit, &limit, sizeof(limit));
+}
+#endif
 }  // namespace fmoe
 
 extern "C" int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* offsets, int64_t rows, int32_t groups,

@@ -142,6 +142,10 @@ cudaError_t launch_grouped_gemm(const GemmLaunch& g, cudaStream_t stream, int* d
 // loaded module; take_* reads and clears the current device's.
 cudaError_t take_grouped_status(int32_t* code);
 cudaError_t take_block_matmul_status(int32_t* code);
+#ifdef FMOE_WAIT_LIMIT_SWITCH
+cudaError_t set_grouped_wait_limit(int64_t cycles);
+cudaError_t set_block_matmul_wait_limit(int64_t cycles);
+#endif
 
 // Tensor map of a row-major array (dims and box innermost first, strides of the outer dimensions in
 // bytes, rank 2 or 3) read in 128-byte-swizzled boxes; what lies outside is filled with zeros.

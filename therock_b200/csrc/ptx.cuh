@@ -74,7 +74,11 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
+#ifdef FMOE_WAIT_LIMIT_SWITCH      // does not wait in hardware, so that no time passes unseen
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+#else
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+#endif
       "selp.u32 %0, 1, 0, p;\n\t"
       "}"
       : "=r"(ok)
@@ -86,20 +90,40 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // Bounded wait.  Gives up (returns false) when another role of this CTA has raised
 // *abort_flag or after ~kWaitLimitCycles; on its own timeout it raises the flag itself.
 constexpr long long kWaitLimitCycles = 4000000000LL;  // about two seconds
+#ifdef FMOE_WAIT_LIMIT_SWITCH
+// A build for tests: the host sets the limit, and every turn of a wait looks at it.
+static __device__ volatile long long g_wait_limit = kWaitLimitCycles;
+constexpr uint32_t kSpinMask = 0u;
+__device__ __forceinline__ long long wait_limit() { return g_wait_limit; }
+#else
+constexpr uint32_t kSpinMask = 0xFFu;
+__device__ __forceinline__ constexpr long long wait_limit() { return kWaitLimitCycles; }
+#endif
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   uint32_t spins = 0;
   while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 0xFFu) == 0) {
+    if ((++spins & kSpinMask) == 0) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > kWaitLimitCycles) {
+      if (clock64() - t0 > wait_limit()) {
         *abort_flag = 1;
         return false;
       }
     }
   }
   return true;
+}
+
+// The way out after a wait has run out, once all roles of the CTA have stopped: what they issued before
+// that (loads into shared memory, MMAs on it and their commits) takes microseconds, and a CTA that left
+// earlier would have it land in its successor's memory.  So it stays for about a millisecond.
+constexpr long long kSettleCycles = 2000000LL;
+__device__ __forceinline__ void settle(const volatile int* abort_flag) {
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kSettleCycles) {}
+  }
 }
 
 // ----------------------------------------------------------------------------- TMA
@@ -292,6 +316,12 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Raises the abort flag of a pair's other CTA: its loads and MMAs work on this CTA's memory too, so both
+// give up, and both settle before they leave.
+__device__ __forceinline__ void raise_in_peer(volatile int* abort_flag) {
+  const uint32_t flag = map_to_rank(smem_u32(const_cast<const int*>(abort_flag)), cluster_ctarank() ^ 1u);
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(flag), "r"(1) : "memory");
+}
 // Arrive on an mbarrier that may live in the peer CTA (cluster-space address).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
@@ -353,9 +383,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
   const long long t0 = clock64();
   uint32_t spins = 0;
   while (!mbar_try_wait_cluster(bar, parity)) {
-    if ((++spins & 0xFFu) == 0) {
+    if ((++spins & kSpinMask) == 0) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > kWaitLimitCycles) {
+      if (clock64() - t0 > wait_limit()) {
         *abort_flag = 1;
         return false;
       }
