@@ -77,3 +77,45 @@ direct()
 assert int(word) == code and torch.equal(out, M.grouped_matmul(x, w, off))
 print("done")
 """)
+
+
+def test_a_tile_may_take_longer_than_a_wait():
+    """A wait for a whole tile covers all of its contraction: its limit grows with the stages, so a sum
+    over any number of rows is finished.  Here one stage may take 0.1 ms and a tile takes more than that.
+    Small whole numbers, so every sum is exact."""
+    run("""
+def same(out, ref):
+    assert torch.equal(out, ref.to(out.dtype)), (out.double() - ref).abs().max()
+def dots(a, b):
+    return sum((a[..., i:i + 65536].double() @ b[..., i:i + 65536].double().mT) for i in range(0, a.shape[-1], 65536))
+long = 1 << 20
+limit(200000)
+for rows in (long, long - 3):
+    x, dy = whole(rows, 8).bfloat16(), whole(rows, 8).bfloat16()
+    off = torch.tensor([0, 5, rows], dtype=torch.int32, device=d)
+    dw = M.grouped_matmul_wgrad(dy, x, off)
+    assert M.operator_status(d) == 0
+    same(dw[1], dots(dy[5:].mT, x[5:].mT))
+off = torch.tensor([0, 40], dtype=torch.int32, device=d)
+x, w = whole(40, long).bfloat16(), whole(1, 8, long).bfloat16()
+y = M.grouped_matmul(x, w, off)
+assert M.operator_status(d) == 0
+same(y, dots(x, w[0]))
+wt = w[0].mT.contiguous()[None]
+dx = M.grouped_matmul_dgrad(x, wt, off)
+assert M.operator_status(d) == 0
+same(dx, dots(x, w[0]))
+del x, w, wt
+byte = lambda t: ((t == 1) * 0x38 + (t == -1) * 0xb8).to(torch.uint8)      # 1 and -1 in e4m3
+m, n, k = 8192, 4096, 1 << 17
+a, b = torch.cat([byte(whole(1024, k)) for _ in range(m // 1024)]), torch.cat([byte(whole(1024, k)) for _ in range(n // 1024)])
+ones = lambda *s: torch.ones(*s, device=d)
+at = torch.tensor([0, 1, 127, 128, 4095, 4096, m - 1], device=d)
+value = lambda t: t.view(torch.float8_e4m3fn).float()
+ref = dots(value(a[at]), value(b))
+for quant, sa in (("block128_ue8m0", torch.full((m, k // 128), 127, dtype=torch.uint8, device=d)), ("block128", ones(m, k // 128))):
+    out = M.matmul_block128(a, sa, b, ones(n // 128, k // 128), quant)
+    assert M.operator_status(d) == 0, quant
+    same(out[at], ref)
+print("done")
+""")

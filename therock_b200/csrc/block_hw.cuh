@@ -263,7 +263,7 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
     for (int tile = first_tile; tile < total_tiles; tile += tile_step) {
       const BlockTile at = decode_block_tile<Cfg::kTileM>(tile, p.m_blocks, p.n_blocks);
       const int m0 = at.m * Cfg::kTileM + static_cast<int>(rank) * kBmmTileM, n0 = at.n * kHwTileN;
-      if (!ptx::mbar_wait(acc_full, phase, abort_flag)) { ok = false; break; }
+      if (!ptx::mbar_wait(acc_full, phase, abort_flag, p.kb)) { ok = false; break; }
       phase ^= 1u;
       ptx::tc_fence_after();
       uint32_t v[4][32];

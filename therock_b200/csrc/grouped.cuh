@@ -337,7 +337,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     bool ok = true;
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const RowsTile t = decode_rows_tile(tile, s.starts, s.cum, p.groups, p.m_blocks);
-      if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag)) { ok = false; break; }
+      if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag, p.k_iters)) { ok = false; break; }
       ptx::tc_fence_after();
       const int col = t.m_blk * kGrpTile + static_cast<int>(rank) * 128 + quad * 32 + (lane & ~1);
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);
@@ -528,7 +528,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       stage = (stage + n_stages) % kWgStages;
       const int live = size - (n_stages - 1) * kGrpStageK;
       if ((live & 15) == 0) continue;
-      if (!ptx::mbar_wait(ptx::smem_u32(&s.tail_bar[last_stage]), (phases >> last_stage) & 1u, s.abort_flag)) { ok = false; break; }
+      if (!ptx::mbar_wait(ptx::smem_u32(&s.tail_bar[last_stage]), (phases >> last_stage) & 1u, s.abort_flag, n_stages)) { ok = false; break; }
       const int end = (live + 15) & ~15;
       uint8_t* st = s.stages + last_stage * kGrpStageBytes;
       // four 64-column chunks (two of dy, two of x) of 64 rows x 128 bytes
@@ -567,9 +567,10 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       const int local = tile - g * per_group;
       const int n0 = local / p.k_blocks * kGrpTile + static_cast<int>(rank) * 128 + quad * 32;
       const int k0 = local % p.k_blocks * kGrpTile;
-      const bool empty = s.starts[g + 1] == s.starts[g];
+      const int size = s.starts[g + 1] - s.starts[g];
+      const bool empty = size == 0;
       if (!empty) {
-        if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag)) { ok = false; break; }
+        if (!ptx::mbar_wait(ptx::smem_u32(&s.acc_full_bar[acc]), acc_phase, s.abort_flag, size / kGrpStageK + 1)) { ok = false; break; }
         ptx::tc_fence_after();
       }
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(acc * kGrpTile);

@@ -89,6 +89,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 
 // Bounded wait.  Gives up (returns false) when another role of this CTA has raised
 // *abort_flag or after ~kWaitLimitCycles; on its own timeout it raises the flag itself.
+// A wait that covers `stages` steps of other roles, each of which has a wait of its own, allows
+// for all of them: a stage takes some 500 cycles (1500 where all SMs load from memory).
 constexpr long long kWaitLimitCycles = 4000000000LL;  // about two seconds
 #ifdef FMOE_WAIT_LIMIT_SWITCH
 // A build for tests: the host sets the limit, and every turn of a wait looks at it.
@@ -99,14 +101,15 @@ __device__ __forceinline__ long long wait_limit() { return g_wait_limit; }
 constexpr uint32_t kSpinMask = 0xFFu;
 __device__ __forceinline__ constexpr long long wait_limit() { return kWaitLimitCycles; }
 #endif
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+constexpr long long kWaitCyclesPerStage = 16384LL;
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int stages = 0) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   uint32_t spins = 0;
   while (!mbar_try_wait(bar, parity)) {
     if ((++spins & kSpinMask) == 0) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > wait_limit()) {
+      if (clock64() - t0 > wait_limit() + stages * kWaitCyclesPerStage) {
         *abort_flag = 1;
         return false;
       }
