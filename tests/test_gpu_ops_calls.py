@@ -1,0 +1,49 @@
+"""Calls of the expert layer's parts beside the plain ones: results given by the caller inside a graph,
+tracers, derivatives of other kinds, hooks on what a graph keeps."""
+import pytest
+import torch
+
+import therock_b200 as M
+from tests.test_gpu_ops import DEV, block_inputs, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls_with_results():
+    """name: (the call, its results' keyword names)"""
+    off = offsets_of([3, 30])
+    x, w = torch.randn(33, 64, device=DEV).bfloat16(), torch.randn(2, 48, 64, device=DEV).bfloat16()
+    dy = torch.randn(33, 48, device=DEV).bfloat16()
+    gu, rw = torch.randn(9, 512, device=DEV).half(), torch.rand(9, device=DEV)
+    q = block_inputs(5, 70, 256, "block128", seed=2)
+    return {"y": (lambda **o: M.grouped_matmul(x, w, off, **o), ("out",)), "dx": (lambda **o: M.grouped_matmul_dgrad(dy, w, off, **o), ("out",)),
+            "dw": (lambda **o: M.grouped_matmul_wgrad(dy, x, off, **o), ("out",)), "silu": (lambda **o: M.silu_mul(gu, rw, **o), ("out",)),
+            "block": (lambda **o: M.matmul_block128(*q, **o), ("out",)),
+            "quantise": (lambda **o: M.silu_mul_quantise(gu, "block128", rw, **o), ("q", "scales"))}
+
+
+@pytest.mark.parametrize("name", ["y", "dx", "dw", "silu", "block", "quantise"])
+def test_a_result_over_a_tensor_that_a_graph_has_saved(name):
+    """The graph's backward pass raises, as it does after any write in place, and does not use the new values."""
+    call, names = _calls_with_results()[name]
+    first = call()
+    results = [torch.empty_like(t) for t in (first if isinstance(first, tuple) else (first,))]
+    leaves = [torch.ones(t.shape, device=DEV, requires_grad=True) for t in results]
+    with torch.no_grad():
+        call(**dict(zip(names, results)))
+    losses = [(leaf * t).sum() for leaf, t in zip(leaves, results)]       # each keeps its result for the leaf's gradient
+    with torch.no_grad():
+        call(**dict(zip(names, results)))
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+@pytest.mark.parametrize("name", ["y", "dx", "dw", "silu", "block"])
+def test_a_result_that_requires_a_gradient_is_refused(name):
+    call, (key,) = _calls_with_results()[name]
+    out = torch.empty_like(call()).requires_grad_()
+    with pytest.raises(M.FmoeError, match="gradient"):
+        call(**{key: out})
+    with torch.no_grad():
+        assert call(**{key: out}) is out

@@ -18,6 +18,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .api import QUANT, FmoeError, _check, lib
 
@@ -116,11 +117,21 @@ def _result(name: str, out, shape, dtype, like: torch.Tensor, stream, *apart) ->
     _dense(name, out, like.get_device())
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise FmoeError(-1, f"{name} must be {dtype} {tuple(shape)}")
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise FmoeError(-1, f"{name} must not require a gradient")
     first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
     for t in apart:
         if t is not None and t.data_ptr() < last and first < t.data_ptr() + t.numel() * t.element_size():
             raise FmoeError(-1, f"{name} must not share memory with the other tensors")
     return out
+
+
+def _filled(given, result):
+    """`result`, with the tensor that the caller gave for it marked as written: a graph that had saved it
+    says so instead of using its new values."""
+    if given is not None:
+        increment_version(given)
+    return result
 
 
 def _for_kernel(t: torch.Tensor) -> torch.Tensor:
@@ -152,12 +163,12 @@ def _grouped(x, weight, offsets, transpose: bool, out, stream):
     groups, n, k = weight.shape
     rows = x.shape[0]
     _sizes(groups, n, k)
-    out = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream, x, weight, offsets)
+    y = _result("out", out, (rows, k if transpose else n), x.dtype, x, stream, x, weight, offsets)
     rc = _bound().fmoe_grouped_matmul(x.data_ptr(), weight.data_ptr(), offsets.data_ptr(), rows, groups, n, k, _DTYPE[x.dtype],
-                                      transpose, out.data_ptr(), None, _stream_of(x, stream))
+                                      transpose, y.data_ptr(), None, _stream_of(x, stream))
     if rc:
         _check(rc)
-    return out
+    return _filled(out, y)
 
 
 def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -191,10 +202,10 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
         raise FmoeError(-1, "offsets must be int32 [groups + 1]")
     groups, n, k = offsets.shape[0] - 1, dy.shape[1], x.shape[1]
     _sizes(groups, n, k)
-    out = _result("out", out, (groups, n, k), x.dtype, x, stream, dy, x, offsets)
+    dw = _result("out", out, (groups, n, k), x.dtype, x, stream, dy, x, offsets)
     _check(_bound().fmoe_grouped_matmul_wgrad(dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), x.shape[0], groups, n, k,
-                                              _DTYPE[x.dtype], out.data_ptr(), None, _stream_of(x, stream)))
-    return out
+                                              _DTYPE[x.dtype], dw.data_ptr(), None, _stream_of(x, stream)))
+    return _filled(out, dw)
 
 
 def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -253,10 +264,10 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     if w_scale.dtype is not torch.float32 or w_scale.shape != ((n + 127) // 128, blocks):
         raise FmoeError(-1, f"w_scale must be float32 [{(n + 127) // 128}, {blocks}]")
     _sizes(n, k)
-    out = _result("out", out, (m, n), torch.bfloat16, a, stream, a, a_scale, w, w_scale)
+    y = _result("out", out, (m, n), torch.bfloat16, a, stream, a, a_scale, w, w_scale)
     _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
-                                         QUANT[quant], out.data_ptr(), None, _stream_of(a, stream)))
-    return out
+                                         QUANT[quant], y.data_ptr(), None, _stream_of(a, stream)))
+    return _filled(out, y)
 
 
 # ----------------------------------------------------------------------------- the gated activation
@@ -276,10 +287,10 @@ def _check_silu(gu, row_weight):
 
 def _silu(gu, row_weight, out, stream):
     rows, width = gu.shape[0], gu.shape[1] // 2
-    out = _result("out", out, (rows, width), gu.dtype, gu, stream, gu, row_weight)
+    y = _result("out", out, (rows, width), gu.dtype, gu, stream, gu, row_weight)
     _check(_bound().fmoe_silu_mul(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
-                                  _DTYPE[gu.dtype], out.data_ptr(), _stream_of(gu, stream)))
-    return out
+                                  _DTYPE[gu.dtype], y.data_ptr(), _stream_of(gu, stream)))
+    return _filled(out, y)
 
 
 def silu_mul_backward(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optional[torch.Tensor] = None, stream=None):
@@ -326,9 +337,9 @@ def silu_mul_quantise(gu: torch.Tensor, quant: str, row_weight: Optional[torch.T
         raise FmoeError(-2, "width must be a multiple of 128")
     groups = width // 128
     row_bytes = 4 * groups if quant == "block128" else (groups + 3) // 4 * 4
-    q = _result("q", q, (rows, width), torch.uint8, gu, stream, gu, row_weight)
-    scales = _result("scales", scales, (rows, row_bytes), torch.uint8, gu, stream, gu, row_weight, q)
+    to = _result("q", q, (rows, width), torch.uint8, gu, stream, gu, row_weight)
+    s = _result("scales", scales, (rows, row_bytes), torch.uint8, gu, stream, gu, row_weight, to)
     _check(_bound().fmoe_silu_mul_quantise(gu.data_ptr(), None if row_weight is None else row_weight.data_ptr(), rows, width,
-                                           _DTYPE[gu.dtype], QUANT[quant], q.data_ptr(), scales.data_ptr(),
+                                           _DTYPE[gu.dtype], QUANT[quant], to.data_ptr(), s.data_ptr(),
                                            _stream_of(gu, stream)))
-    return q, scales
+    return _filled(q, to), _filled(scales, s)
