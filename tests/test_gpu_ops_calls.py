@@ -2,6 +2,7 @@
 tracers, derivatives of other kinds, hooks on what a graph keeps."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import therock_b200 as M
 from tests.test_gpu_ops import DEV, block_inputs, offsets_of
@@ -47,3 +48,22 @@ def test_a_result_that_requires_a_gradient_is_refused(name):
         call(**{key: out})
     with torch.no_grad():
         assert call(**{key: out}) is out
+
+
+@pytest.mark.parametrize("recording", [True, False])
+@pytest.mark.parametrize("second", [False, True])
+@pytest.mark.parametrize("name", ["grouped", "silu"])
+def test_a_tangent_is_not_dropped(name, second, recording):
+    """Forward-mode derivatives are recorded under torch.no_grad too, so the call is refused there as well,
+    with a result given by the caller or without."""
+    off = offsets_of([10, 0, 23])
+    x, w, rw = torch.randn(33, 64, device=DEV).bfloat16(), torch.randn(3, 32, 64, device=DEV).bfloat16(), torch.rand(33, device=DEV)
+    f, inputs = (lambda a, b, **o: M.grouped_matmul(a, b, off, **o), [x, w]) if name == "grouped" else (M.silu_mul, [x, rw])
+    out = f(*inputs)
+    with fwd.dual_level(), torch.set_grad_enabled(recording):
+        inputs[second] = fwd.make_dual(inputs[second], torch.ones_like(inputs[second]))
+        for o in ({}, {"out": out}):
+            with pytest.raises(M.FmoeError, match="forward-mode"):
+                f(*inputs, **o)
+        with fwd._set_fwd_grad_enabled(False):
+            assert torch.equal(f(*inputs), out)

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
@@ -63,7 +64,11 @@ bool fits32(const at::Tensor& t) {
     if (d > INT32_MAX) return false;
   return true;
 }
-bool differentiable(const at::Tensor& t) { return t.requires_grad() || t._fw_grad(0).defined(); }
+// Forward-mode derivatives go by a mode of their own: torch.no_grad does not switch them off.
+void refuse_tangent(const at::Tensor& t) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    throw Failure(FMOE_ERR_INVALID_ARG, "forward-mode derivatives are not supported");
+}
 
 // A backward pass that is being captured cannot hand gradients to a node of the default stream, which
 // cannot join a capture: a leaf has such a node as long as any earlier graph of it lives.  The engine
@@ -204,10 +209,12 @@ PyObject* py_grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *x, *w, *off;
   if (n != 3 || !(x = tensor(args[0])) || !(w = tensor(args[1])) || !(off = tensor(args[2])) || !grouped_fits(*x, *w, *off))
     Py_RETURN_NONE;
+  refuse_tangent(*x);
+  refuse_tangent(*w);
   at::Tensor out;
   {
     Unlocked unlocked;
-    out = at::GradMode::is_enabled() && (differentiable(*x) || differentiable(*w)) ? GroupedMatmul::apply(*x, *w, *off)
+    out = at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad()) ? GroupedMatmul::apply(*x, *w, *off)
                                                                                    : grouped(*x, *w, *off, false);
   }
   return THPVariable_Wrap(std::move(out));
@@ -254,10 +261,12 @@ PyObject* py_silu_mul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* gu;
   std::optional<at::Tensor> weight;
   if (n != 2 || !(gu = tensor(args[0])) || !weight_of(args[1], &weight) || !silu_fits(*gu, weight)) Py_RETURN_NONE;
+  refuse_tangent(*gu);
+  if (weight) refuse_tangent(*weight);
   at::Tensor out;
   {
     Unlocked unlocked;
-    out = at::GradMode::is_enabled() && (differentiable(*gu) || (weight && differentiable(*weight))) ? SiluMul::apply(*gu, weight)
+    out = at::GradMode::is_enabled() && (gu->requires_grad() || (weight && weight->requires_grad())) ? SiluMul::apply(*gu, weight)
                                                                                                     : silu(*gu, weight);
   }
   return THPVariable_Wrap(std::move(out));

@@ -18,6 +18,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from .api import QUANT, FmoeError, _check, lib
@@ -143,6 +144,8 @@ def _for_kernel(t: torch.Tensor) -> torch.Tensor:
 def _refuse_gradients(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise FmoeError(-1, "forward-mode derivatives are not supported")
 
 
 # ----------------------------------------------------------------------------- products grouped by expert
