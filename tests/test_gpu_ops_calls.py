@@ -67,3 +67,54 @@ def test_a_tangent_is_not_dropped(name, second, recording):
                 f(*inputs, **o)
         with fwd._set_fwd_grad_enabled(False):
             assert torch.equal(f(*inputs), out)
+
+
+def _layer(name):
+    import therock_b200.torch_op  # noqa: F401
+    off = offsets_of([10, 0, 23])
+    op = M.grouped_matmul if name == "M" else torch.ops.therock_b200.grouped_matmul
+    x, w = (torch.randn(*s, device=DEV).bfloat16().requires_grad_() for s in ((33, 64), (3, 96, 64)))
+    return x, w, lambda x, w: op(x, w, off), torch.randn(33, 96, device=DEV).bfloat16()
+
+
+@pytest.mark.parametrize("name", ["M", "op"])
+def test_a_captured_backward_pass_beside_a_living_graph_of_a_leaf_further_on(name):
+    """The leaf whose node is on the default stream lies behind another operation."""
+    x, w, f, dy = _layer(name)
+    w.requires_grad_(False)
+    living = x.exp()
+
+    def step():
+        return torch.autograd.grad(f(x.neg(), w), x, dy)[0]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(g):
+            step()
+    del living, g
+    want = step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("name", ["M", "op"])
+def test_a_captured_backward_pass_that_leaves_a_living_graphs_leaf_alone(name):
+    """A gradient that the pass does not ask for stands in nobody's way."""
+    x, w, f, dy = _layer(name)
+    living = f(x.detach(), w)
+
+    def step():
+        return torch.autograd.grad(f(x, w), x, dy)[0]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(step(), got)
+    (dw,) = torch.autograd.grad(living, w, dy)
+    assert torch.equal(dw, M.grouped_matmul_wgrad(dy, x.detach(), offsets_of([10, 0, 23])))

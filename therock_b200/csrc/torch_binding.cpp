@@ -16,6 +16,9 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <unordered_set>
+#include <vector>
+
 #include "../../include/fused_moe_c.h"
 
 namespace {
@@ -72,19 +75,29 @@ void refuse_tangent(const at::Tensor& t) {
 
 // A backward pass that is being captured cannot hand gradients to a node of the default stream, which
 // cannot join a capture: a leaf has such a node as long as any earlier graph of it lives.  The engine
-// would break the capture, and with it the process; this ends the pass with an error instead.
+// would break the capture, and with it the process; this ends the pass with an error instead.  It looks
+// at every node that the rest of this pass reaches from here, and at no other.
 void refuse_default_stream_in_capture(int device) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
   if (!node) return;
   const c10::Stream blocked = c10::cuda::getDefaultCUDAStream(static_cast<c10::DeviceIndex>(device)).unwrap();
-  for (const auto& edge : node->next_edges()) {
-    if (!edge.is_valid()) continue;
-    const std::optional<c10::Stream> s = edge.function->stream();
-    if (s && *s == blocked)
-      throw std::runtime_error(
-          "a backward pass is being captured in a CUDA graph while an earlier graph of the same tensors, recorded "
-          "on the default stream, is alive: drop its results (or record it on a side stream) before the capture");
+  std::vector<torch::autograd::Node*> left{node.get()};
+  std::unordered_set<torch::autograd::Node*> seen{node.get()};
+  while (!left.empty()) {
+    torch::autograd::Node* at = left.back();
+    left.pop_back();
+    for (uint32_t i = 0; i < at->num_outputs(); ++i) {
+      if (!at->task_should_compute_output(i)) continue;
+      torch::autograd::Node* next = at->next_edge(i).function.get();
+      if (!seen.insert(next).second) continue;
+      const std::optional<c10::Stream> s = next->stream();
+      if (s && *s == blocked)
+        throw std::runtime_error(
+            "a backward pass is being captured in a CUDA graph while an earlier graph of the same tensors, recorded "
+            "on the default stream, is alive: drop its results (or record it on a side stream) before the capture");
+      left.push_back(next);
+    }
   }
 }
 
