@@ -118,3 +118,46 @@ def test_a_captured_backward_pass_that_leaves_a_living_graphs_leaf_alone(name):
     assert torch.equal(step(), got)
     (dw,) = torch.autograd.grad(living, w, dy)
     assert torch.equal(dw, M.grouped_matmul_wgrad(dy, x.detach(), offsets_of([10, 0, 23])))
+
+
+def _saved_through(give_back):
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, give_back)
+
+
+@pytest.mark.parametrize("which", ["grouped", "silu"])
+def test_what_a_graph_kept_may_come_back_with_other_strides(which):
+    x, w, f, dy = _layer("M")
+    rw = torch.rand(33, device=DEV).requires_grad_()
+    leaves, f, dy = ([x, w], f, dy) if which == "grouped" else ([x, rw], M.silu_mul, dy[:, :32].contiguous())
+    want = torch.autograd.grad(f(*leaves), leaves, dy)
+
+    def strided(t):
+        return t if t.dim() < 2 else t.mT.contiguous().mT
+    with _saved_through(strided):
+        y = f(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
+@pytest.mark.parametrize("which", ["grouped", "silu"])
+@pytest.mark.parametrize("index", [0, 1, 2])
+@pytest.mark.parametrize("change", ["shorter", "wider type", "host", "flat"])
+def test_what_a_graph_kept_is_checked_when_it_comes_back(change, index, which):
+    """A hook that gives back something else ends the pass; nothing is read by the old sizes."""
+    x, w, f, dy = _layer("M")
+    rw = torch.rand(33, device=DEV).requires_grad_()
+    leaves, f, dy = ([x, w], f, dy) if which == "grouped" else ([x, rw], M.silu_mul, dy[:, :32].contiguous())
+    how = {"shorter": lambda t: t[:-1], "wider type": lambda t: t.double(), "host": lambda t: t.cpu(), "flat": lambda t: t[None]}[change]
+    given = []
+
+    def give_back(t):
+        given.append(t)
+        return how(t.detach()) if len(given) == index + 1 else t
+    with _saved_through(give_back):
+        y = f(*leaves)
+    if which == "silu" and index == 2:
+        torch.autograd.grad(y, leaves, dy)
+        assert len(given) == 2
+        return
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaves, dy)
+    torch.cuda.synchronize()

@@ -101,10 +101,17 @@ void refuse_default_stream_in_capture(int device) {
   }
 }
 
-// A gradient that autograd may hand over with any strides, as the kernels read it.
+// A gradient that autograd may hand over with any strides, or a tensor that a hook on saved tensors gave
+// back, as the kernels read it.
 at::Tensor for_kernel(const at::Tensor& t) {
   at::Tensor c = t.contiguous();
   return aligned(c, 16) ? c : c.clone();
+}
+
+bool same_kind(const at::Tensor& a, const at::Tensor& b) { return a.scalar_type() == b.scalar_type() && a.get_device() == b.get_device(); }
+// What a graph kept comes back through the user's hooks, if there are any, and is checked like an argument.
+[[noreturn]] void throw_not_saved() {
+  throw Failure(FMOE_ERR_INVALID_ARG, "what came back from a hook on saved tensors is not what was saved (type, shape or device)");
 }
 
 // Gradients are first order: what a backward pass with create_graph = True returns raises when it is
@@ -145,12 +152,12 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &w = saved[1], &off = saved[2];
-    refuse_default_stream_in_capture(x.get_device());
+    refuse_default_stream_in_capture(grads[0].get_device());
     torch::autograd::variable_list out(3);
     {
       at::NoGradGuard no_grad;
-      const at::Tensor dy = for_kernel(grads[0]);
+      const at::Tensor dy = for_kernel(grads[0]), x = for_kernel(saved[0]), w = for_kernel(saved[1]), off = for_kernel(saved[2]);
+      if (!grouped_fits(x, w, off) || !same_kind(x, dy) || dy.size(0) != x.size(0) || dy.size(1) != w.size(1)) throw_not_saved();
       if (ctx->needs_input_grad(0)) out[0] = grouped(dy, w, off, true);
       if (ctx->needs_input_grad(1)) {
         out[1] = at::empty(w.sizes(), w.options().requires_grad(false));
@@ -187,12 +194,15 @@ struct SiluMul : torch::autograd::Function<SiluMul> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &gu = saved[0], &weight = saved[1];
-    refuse_default_stream_in_capture(gu.get_device());
+    refuse_default_stream_in_capture(grads[0].get_device());
     torch::autograd::variable_list out(2);
     {
       at::NoGradGuard no_grad;
-      const at::Tensor dy = for_kernel(grads[0]);
+      const at::Tensor dy = for_kernel(grads[0]), gu = for_kernel(saved[0]);
+      const at::Tensor weight = saved[1].defined() ? for_kernel(saved[1]) : at::Tensor();
+      if (!silu_fits(gu, weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt) || !same_kind(gu, dy) ||
+          dy.size(0) != gu.size(0) || 2 * dy.size(1) != gu.size(1))
+        throw_not_saved();
       out[0] = at::empty(gu.sizes(), gu.options().requires_grad(false));
       if (weight.defined()) out[1] = at::empty(weight.sizes(), weight.options().requires_grad(false));
       check(F.silu_backward(gu.data_ptr(), weight.defined() ? weight.data_ptr<float>() : nullptr, dy.data_ptr(), gu.size(0),
