@@ -161,3 +161,61 @@ def test_what_a_graph_kept_is_checked_when_it_comes_back(change, index, which):
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y, leaves, dy)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("name", ["y", "dx", "dw", "silu", "silu gradients", "block", "quantise"])
+def test_a_tracer_does_not_record_an_empty_result(name):
+    """make_fx and torch.jit.trace would see the allocation of the result only; the call is refused, with a
+    result given by the caller too.  It is as good as ever under a mode that records nothing."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    if name == "silu gradients":
+        gu, dy = torch.randn(9, 512, device=DEV).half(), torch.randn(9, 256, device=DEV).half()
+        call, names = lambda: M.silu_mul_backward(gu, dy)[0], ()
+    else:
+        call, names = _calls_with_results()[name]
+    want = call()
+    x = torch.ones(3, device=DEV)
+    given = [{}] + [dict(zip(names, want if isinstance(want, tuple) else (want,)))] * bool(names)
+    for out in given:
+        def program(x):
+            r = call(**out)
+            return (r[0] if isinstance(r, tuple) else r) + x[0]
+        for trace in (lambda: make_fx(program)(x), lambda: make_fx(program, pre_dispatch=True)(x), lambda: torch.jit.trace(program, (x,), check_trace=False)):
+            with pytest.raises(M.FmoeError, match="traced program"):
+                trace()
+        with FlopCounterMode(display=False):
+            program(x)
+
+
+def test_traced_and_compiled_programs_hold_the_registered_operators():
+    import therock_b200.torch_op  # noqa: F401
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ns = torch.ops.therock_b200
+    x, w, _, _ = _layer("M")
+    off = offsets_of([10, 0, 23])
+    q = block_inputs(33, 70, 256, "block128", seed=2)
+
+    def layer(x, w, off, *q):
+        return ns.silu_mul(ns.grouped_matmul(x, w, off)).float().square().sum() + ns.matmul_block128(*q).float().sum()
+    rest = (off, *q)
+    with torch.no_grad():
+        for program in (make_fx(layer)(x, w, *rest), torch.jit.trace(layer, (x, w, *rest), check_trace=False),
+                        make_fx(layer, tracing_mode="fake")(x, w, *rest)):
+            assert torch.equal(program(-x, w, *rest), layer(-x, w, *rest))
+    compiled = torch.compile(layer, backend="aot_eager", fullgraph=True, dynamic=True)
+    want, got = torch.autograd.grad(layer(x, w, *rest), (x, w)), torch.autograd.grad(compiled(x, w, *rest), (x, w))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("name", ["grouped_matmul", "grouped_matmul_dgrad", "grouped_matmul_wgrad", "matmul_block128", "silu_mul", "silu_mul_backward"])
+def test_registered_operators_pass_opcheck(name):
+    import therock_b200.torch_op  # noqa: F401
+    x, w, _, dy = _layer("M")
+    off, rw = offsets_of([10, 0, 23]), torch.rand(33, device=DEV).requires_grad_()
+    a, sa, b, sb = block_inputs(33, 70, 256, "block128", seed=2)
+    calls = {"grouped_matmul": [(x, w, off)], "grouped_matmul_dgrad": [(dy, w.detach(), off)], "grouped_matmul_wgrad": [(dy, x.detach(), off)],
+             "matmul_block128": [(a, sa, b.view(torch.uint8), sb)], "silu_mul": [(x,), (x, rw)],
+             "silu_mul_backward": [(x.detach(), dy[:, :32].contiguous()), (x.detach(), dy[:, :32].contiguous(), rw.detach())]}
+    for args in calls[name]:
+        assert set(torch.library.opcheck(getattr(torch.ops.therock_b200, name).default, args).values()) == {"SUCCESS"}

@@ -12,6 +12,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
@@ -225,12 +227,20 @@ PyObject* raise(const Failure& f) {
 #define FMOE_TRY HANDLE_TH_ERRORS try {
 #define FMOE_CATCH } catch (const Failure& f) { return raise(f); } END_HANDLE_TH_ERRORS
 
+// True while a tracer records what runs (make_fx, torch.jit.trace, export): it would see the allocation of
+// the result and nothing else.  Inside a registered operator, whose call it records, it is off.
+bool traced() {
+  auto on = [](at::DispatchKey k) { return c10::impl::tls_is_dispatch_key_included(k) && !c10::impl::tls_is_dispatch_key_excluded(k); };
+  return c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+         on(at::DispatchKey::Tracer) || on(at::DispatchKey::PreDispatch);
+}
+
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 PyObject* py_grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FMOE_TRY
   const at::Tensor *x, *w, *off;
-  if (n != 3 || !(x = tensor(args[0])) || !(w = tensor(args[1])) || !(off = tensor(args[2])) || !grouped_fits(*x, *w, *off))
+  if (n != 3 || traced() || !(x = tensor(args[0])) || !(w = tensor(args[1])) || !(off = tensor(args[2])) || !grouped_fits(*x, *w, *off))
     Py_RETURN_NONE;
   refuse_tangent(*x);
   refuse_tangent(*w);
@@ -247,7 +257,7 @@ PyObject* py_grouped_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_matmul_block128(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FMOE_TRY
   const at::Tensor *a, *sa, *w, *sw;
-  if (n != 5 || !(a = tensor(args[0])) || !(sa = tensor(args[1])) || !(w = tensor(args[2])) || !(sw = tensor(args[3]))) Py_RETURN_NONE;
+  if (n != 5 || traced() || !(a = tensor(args[0])) || !(sa = tensor(args[1])) || !(w = tensor(args[2])) || !(sw = tensor(args[3]))) Py_RETURN_NONE;
   const bool hw = PyLong_AsLong(args[4]) == FMOE_QUANT_BLOCK128_UE8M0;
   if (!(dense(*a) && dense(*w) && dense(*sa, 4) && dense(*sw, 4) && byte_type(a->scalar_type()) && byte_type(w->scalar_type()) &&
         a->dim() == 2 && w->dim() == 2 && a->size(1) == w->size(1) && sa->dim() == 2 && sw->dim() == 2)) 
@@ -283,7 +293,7 @@ PyObject* py_silu_mul(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FMOE_TRY
   const at::Tensor* gu;
   std::optional<at::Tensor> weight;
-  if (n != 2 || !(gu = tensor(args[0])) || !weight_of(args[1], &weight) || !silu_fits(*gu, weight)) Py_RETURN_NONE;
+  if (n != 2 || traced() || !(gu = tensor(args[0])) || !weight_of(args[1], &weight) || !silu_fits(*gu, weight)) Py_RETURN_NONE;
   refuse_tangent(*gu);
   if (weight) refuse_tangent(*weight);
   at::Tensor out;
@@ -300,7 +310,7 @@ PyObject* py_silu_mul_quantise(PyObject*, PyObject* const* args, Py_ssize_t n) {
   FMOE_TRY
   const at::Tensor* gu;
   std::optional<at::Tensor> weight;
-  if (n != 3 || !(gu = tensor(args[0])) || !weight_of(args[2], &weight) || !silu_fits(*gu, weight) || gu->size(1) % 256 != 0)
+  if (n != 3 || traced() || !(gu = tensor(args[0])) || !weight_of(args[2], &weight) || !silu_fits(*gu, weight) || gu->size(1) % 256 != 0)
     Py_RETURN_NONE;
   const bool hw = PyLong_AsLong(args[1]) == FMOE_QUANT_BLOCK128_UE8M0;
   const int64_t rows = gu->size(0), width = gu->size(1) / 2, groups = width / 128;

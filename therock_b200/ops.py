@@ -11,7 +11,8 @@ returns: no host synchronisation, no atomics, so the same inputs give the same b
 be captured in a CUDA graph (a forward and its backward pass in one graph; no earlier graph of the
 same tensors that was recorded on the default stream may be alive).  Inputs are contiguous CUDA tensors on one device, which need not be
 the current one; a call on another stream than the current one allocates its results for that
-stream, and the caller orders the streams.  Bad arguments raise FmoeError before any launch."""
+stream, and the caller orders the streams.  Bad arguments raise FmoeError before any launch, and so does a
+call that a tracer records (torch.ops.therock_b200 has the operators for traced and compiled programs)."""
 from __future__ import annotations
 
 import ctypes
@@ -141,6 +142,18 @@ def _for_kernel(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() & 15 else t
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_TRACERS = [torch._C._dispatch_key_parse(k) for k in ("Tracer", "PreDispatch")]
+
+
+def _refuse_tracers() -> None:
+    """A tracer (make_fx, torch.jit.trace, export) would record the allocation of the result and not the
+    call that fills it.  Inside a registered operator it is off."""
+    if torch._C._get_dispatch_mode(_PROXY) is not None or any(
+            torch._C._dispatch_tls_is_dispatch_key_included(k) and not torch._C._dispatch_tls_is_dispatch_key_excluded(k) for k in _TRACERS):
+        raise FmoeError(-1, "a traced program cannot hold this call: use torch.ops.therock_b200 (import therock_b200.torch_op)")
+
+
 def _refuse_gradients(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
@@ -150,6 +163,7 @@ def _refuse_gradients(*tensors) -> None:
 
 # ----------------------------------------------------------------------------- products grouped by expert
 def _check_grouped(x, weight, offsets):
+    _refuse_tracers()
     index = _dense("x", x)
     _dense("weight", weight, index)
     _dense("offsets", offsets, index, 4)
@@ -178,6 +192,7 @@ def grouped_matmul_dgrad(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.
                          stream=None) -> torch.Tensor:
     """dx [rows, k] with dx[r] = weight[g]^T dy[r] for the rows of group g, zeros for rows of none: the
     gradient of grouped_matmul with respect to x, from dy [rows, n].  No gradient of its own."""
+    _refuse_tracers()
     index = _dense("dy", dy)
     _dense("weight", weight, index)
     _dense("offsets", offsets, index, 4)
@@ -194,6 +209,7 @@ def grouped_matmul_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
                          stream=None) -> torch.Tensor:
     """dw [groups, n, k] with dw[g] = dy[rows of g]^T x[rows of g]; zeros for a group without rows.
     Rows of no group do not enter it, whatever they hold.  No gradient of its own."""
+    _refuse_tracers()
     index = _dense("dy", dy)
     _dense("x", x, index)
     _dense("offsets", offsets, index, 4)
@@ -246,6 +262,7 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
         y = (_binding or _native()).matmul_block128(a, a_scale, w, w_scale, QUANT[quant])
         if y is not None:
             return y
+    _refuse_tracers()
     index = _dense("a", a)
     _dense("w", w, index)
     if a.dtype not in _E4M3 or w.dtype not in _E4M3:
@@ -275,6 +292,7 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
 
 # ----------------------------------------------------------------------------- the gated activation
 def _check_silu(gu, row_weight):
+    _refuse_tracers()
     index = _dense("gu", gu)
     if gu.dtype not in _DTYPE:
         raise FmoeError(-1, "gu must be bfloat16 or float16")
