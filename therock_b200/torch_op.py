@@ -42,6 +42,39 @@ def _(logits, topk, mode="softmax"):
 
 
 # ----------------------------------------------------------------------------- the parts of an expert layer
+# The fake implementations refuse what the operators refuse by type, shape and layout.
+def _fake_grouped(rows, weight, offsets, dim):
+    torch._check(rows.dim() == 2 and weight.dim() == 3 and offsets.dim() == 1, lambda: "rows must be a matrix, weight [groups, n, k], offsets [groups + 1]")
+    torch._check(rows.dtype in ops._DTYPE and weight.dtype == rows.dtype and offsets.dtype == torch.int32,
+                 lambda: "rows and weight must both be bfloat16 or both float16, offsets int32")
+    torch._check(rows.shape[1] == weight.shape[dim], lambda: "rows and weight do not fit each other")
+    torch._check(offsets.shape[0] == weight.shape[0] + 1, lambda: "offsets must have one more element than there are groups")
+    _fake_widths(weight.shape[1], weight.shape[2])
+    _fake_dense(weight, offsets)
+
+
+def _fake_widths(*widths):
+    for n in widths:
+        torch._check(n > 0, lambda: "a width must not be zero")
+        torch._check(n % 8 == 0, lambda: "n, k and width must be multiples of 8")
+
+
+def _fake_dense(*tensors):
+    for t in tensors:
+        torch._check(t.is_contiguous(), lambda: "tensors must be contiguous")
+
+
+def _fake_silu(gu, row_weight):
+    torch._check(gu.dim() == 2 and gu.dtype in ops._DTYPE, lambda: "gu must be [rows, 2 * width] in bfloat16 or float16")
+    torch._check(gu.shape[1] % 2 == 0, lambda: "gu must be [rows, 2 * width]")
+    _fake_widths(gu.shape[1] // 2)
+    _fake_dense(gu)
+    if row_weight is not None:
+        torch._check(row_weight.dim() == 1 and row_weight.dtype == torch.float32, lambda: "row_weight must be float32 [rows]")
+        torch._check(row_weight.shape[0] == gu.shape[0], lambda: "row_weight must be float32 [rows]")
+        _fake_dense(row_weight)
+
+
 @torch.library.custom_op("therock_b200::grouped_matmul", mutates_args=(), device_types="cuda")
 def grouped_matmul_op(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     return ops.grouped_matmul(x, weight, offsets)
@@ -49,6 +82,8 @@ def grouped_matmul_op(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tens
 
 @grouped_matmul_op.register_fake
 def _(x, weight, offsets):
+    _fake_grouped(x, weight, offsets, 2)
+    _fake_dense(x)
     return x.new_empty(x.shape[0], weight.shape[1])
 
 
@@ -59,6 +94,7 @@ def grouped_matmul_dgrad_op(dy: torch.Tensor, weight: torch.Tensor, offsets: tor
 
 @grouped_matmul_dgrad_op.register_fake
 def _(dy, weight, offsets):
+    _fake_grouped(dy, weight, offsets, 1)
     return dy.new_empty(dy.shape[0], weight.shape[2])
 
 
@@ -69,6 +105,13 @@ def grouped_matmul_wgrad_op(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Te
 
 @grouped_matmul_wgrad_op.register_fake
 def _(dy, x, offsets):
+    torch._check(dy.dim() == 2 and x.dim() == 2 and offsets.dim() == 1, lambda: "dy must be [rows, n], x [rows, k], offsets [groups + 1]")
+    torch._check(x.dtype in ops._DTYPE and dy.dtype == x.dtype and offsets.dtype == torch.int32,
+                 lambda: "dy and x must both be bfloat16 or both float16, offsets int32")
+    torch._check(dy.shape[0] == x.shape[0], lambda: "dy and x must have the same rows")
+    torch._check(offsets.shape[0] >= 2, lambda: "offsets must be int32 [groups + 1]")
+    _fake_widths(dy.shape[1], x.shape[1])
+    _fake_dense(x, offsets)
     return dy.new_empty(offsets.shape[0] - 1, dy.shape[1], x.shape[1])
 
 
@@ -101,6 +144,20 @@ def matmul_block128_op(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
 
 @matmul_block128_op.register_fake
 def _(a, a_scale, w, w_scale, quant="block128"):
+    torch._check(quant in ops._BLOCK_QUANT, lambda: f"quant must be one of {ops._BLOCK_QUANT}")
+    torch._check(a.dtype in ops._E4M3 and w.dtype in ops._E4M3 and w_scale.dtype == torch.float32, lambda: "a and w must be e4m3, w_scale float32")
+    torch._check(a_scale.dtype == torch.uint8 or (a_scale.dtype == torch.float32 and quant == "block128"), lambda: "a_scale must be as quantise_rows returns it")
+    torch._check(a.dim() == 2 and w.dim() == 2 and a_scale.dim() == 2 and w_scale.dim() == 2, lambda: "a, a_scale, w and w_scale must be matrices")
+    torch._check(a.shape[1] == w.shape[1], lambda: "a must be [m, k] and w [n, k]")
+    torch._check(a.shape[1] > 0 and w.shape[0] > 0, lambda: "n and k must not be zero")
+    torch._check(a.shape[1] % 128 == 0, lambda: "k must be a multiple of 128")
+    blocks = a.shape[1] // 128
+    row_bytes = 4 * blocks if quant == "block128" else (blocks + 3) // 4 * 4
+    torch._check(a_scale.shape[0] == a.shape[0], lambda: "a_scale must have a's rows")
+    torch._check(a_scale.shape[1] * a_scale.element_size() == row_bytes, lambda: "a_scale must be as quantise_rows returns it")
+    torch._check(w_scale.shape[0] == (w.shape[0] + 127) // 128, lambda: "w_scale must be [ceil(n / 128), k / 128]")
+    torch._check(w_scale.shape[1] == blocks, lambda: "w_scale must be [ceil(n / 128), k / 128]")
+    _fake_dense(a, a_scale, w, w_scale)
     return a.new_empty(a.shape[0], w.shape[0], dtype=torch.bfloat16)
 
 
@@ -111,6 +168,7 @@ def silu_mul_op(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None) -> 
 
 @silu_mul_op.register_fake
 def _(gu, row_weight=None):
+    _fake_silu(gu, row_weight)
     return gu.new_empty(gu.shape[0], gu.shape[1] // 2)
 
 
@@ -122,6 +180,10 @@ def silu_mul_backward_op(gu: torch.Tensor, dy: torch.Tensor, row_weight: Optiona
 
 @silu_mul_backward_op.register_fake
 def _(gu, dy, row_weight=None):
+    _fake_silu(gu, row_weight)
+    torch._check(dy.dim() == 2 and dy.dtype == gu.dtype, lambda: "dy must be [rows, width] of gu's type")
+    torch._check(dy.shape[0] == gu.shape[0], lambda: "dy must be [rows, width] of gu's type")
+    torch._check(2 * dy.shape[1] == gu.shape[1], lambda: "dy must be [rows, width] of gu's type")
     return torch.empty_like(gu), gu.new_empty(0 if row_weight is None else gu.shape[0], dtype=torch.float32)
 
 
