@@ -57,7 +57,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
 
     src = os.path.join(CSRC, "torch_binding.cpp")
     out = os.path.join(HERE, "_fmoe_torch.so")
-    if not force and not _stale(out, [src, os.path.join(HERE, "..", "include", "fused_moe_c.h")]):
+    made_for = os.path.join(OBJ_DIR, "_fmoe_torch.made_for")
+    if not force and not _stale(out, [src, os.path.join(HERE, "..", "include", "fused_moe_c.h")]) and _recorded(made_for) == _binding_made_for():
         return out
     cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda"
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -72,7 +73,25 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
         print(r.stdout)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for torch_binding.cpp")
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(made_for, "w") as f:
+        f.write(_binding_made_for())
     return out
+
+
+def _binding_made_for() -> str:
+    """What the binding is compiled against: it loads with no other torch or interpreter."""
+    import torch
+
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def _recorded(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
 
 
 def _build_variant(suffix: str, defines: list, force: bool, verbose: bool) -> str:

@@ -58,7 +58,7 @@ def _native():
             from . import _fmoe_torch as binding
         except ImportError as e:
             raise FmoeError(-100, f"the torch binding is missing or does not load ({e}): build it with "
-                                  "`python -m therock_b200.build`") from None
+                                  "`python -m therock_b200.build` under this interpreter and torch") from None
         binding.bind(FmoeError, *(ctypes.cast(getattr(l, n), ctypes.c_void_p).value for n in (
             "fmoe_grouped_matmul", "fmoe_grouped_matmul_wgrad", "fmoe_matmul_block128", "fmoe_silu_mul",
             "fmoe_silu_mul_quantise", "fmoe_silu_mul_backward", "fmoe_last_error")))
