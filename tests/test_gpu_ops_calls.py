@@ -219,3 +219,37 @@ def test_registered_operators_pass_opcheck(name):
              "silu_mul_backward": [(x.detach(), dy[:, :32].contiguous()), (x.detach(), dy[:, :32].contiguous(), rw.detach())]}
     for args in calls[name]:
         assert set(torch.library.opcheck(getattr(torch.ops.therock_b200, name).default, args).values()) == {"SUCCESS"}
+
+
+def test_the_first_calls_of_a_process_may_come_from_several_threads():
+    """Set-up that a first call does (attributes of kernels, occupancy) is shared between threads."""
+    import subprocess
+    import sys
+    text = """
+import threading, torch, therock_b200 as M
+d = "cuda:0"
+torch.manual_seed(0)
+off = torch.tensor([0, 5, 33], dtype=torch.int32, device=d)
+x, w = torch.randn(33, 64, device=d).bfloat16(), torch.randn(2, 256, 64, device=d).bfloat16()
+dy = torch.randn(33, 256, device=d).bfloat16()
+a, b = torch.randn(2100, 1024, device=d).to(torch.float8_e4m3fn), torch.randn(2048, 1024, device=d).to(torch.float8_e4m3fn)
+sa, sb = torch.rand(2100, 8, device=d), torch.rand(16, 8, device=d)
+torch.cuda.synchronize()
+def calls():
+    return [M.grouped_matmul(x, w, off), M.grouped_matmul_dgrad(dy, w, off), M.grouped_matmul_wgrad(dy, x, off), M.silu_mul(dy),
+            M.matmul_block128(a, sa, b, sb), M.matmul_block128(a[:3], sa[:3], b, sb)]
+start, got = threading.Barrier(8), [None] * 8
+def work(i):
+    start.wait()
+    with torch.cuda.stream(torch.cuda.Stream(d)):
+        got[i] = calls()
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+for t in threads: t.start()
+for t in threads: t.join()
+want = calls()
+assert all(torch.equal(p, q) for g in got for p, q in zip(g, want))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]

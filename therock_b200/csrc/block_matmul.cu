@@ -21,26 +21,26 @@ CUresult byte_map(CUtensorMap* tm, const void* base, int64_t rows, int cols, int
 }
 
 template <typename Kernel>
-cudaError_t launch_tiles(Kernel kernel, bool (&configured)[kMaxDevices], int threads, int smem, int cluster, const CUtensorMap& a,
+cudaError_t launch_tiles(Kernel kernel, std::atomic<bool> (&configured)[kMaxDevices], int threads, int smem, int cluster, const CUtensorMap& a,
                          const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
+    if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
   }
   return launch_pdl_cluster(kernel, dim3(grid), dim3(threads), smem, cluster, stream, a, w, p);
 }
 template <bool kPair>
 cudaError_t launch_f32(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices] = {};
   return launch_tiles(fmoe_matmul_block128_kernel<kPair>, configured, kBmmThreads, BmmCfg<kPair>::kSmemBytes, kPair ? 2 : 1, a, w, p,
                       grid, stream);
 }
 template <bool kPair>
 cudaError_t launch_hw(const CUtensorMap& a, const CUtensorMap& w, const BlockMatmulParams& p, int grid, cudaStream_t stream) {
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices] = {};
   return launch_tiles(fmoe_matmul_block128_hw_kernel<kPair>, configured, kHwThreads, HwCfg<kPair>::kSmemBytes, kPair ? 2 : 1, a, w, p,
                       grid, stream);
 }

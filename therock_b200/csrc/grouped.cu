@@ -1,4 +1,6 @@
 // Host side of the products grouped by expert: checks, tensor maps, launches.
+#include <atomic>
+
 #include "grouped.cuh"
 
 #include "host.cuh"
@@ -50,26 +52,26 @@ CUresult weight_map(CUtensorMap* tm, int dtype, const void* base, int groups, in
 }
 
 template <typename Kernel, typename... Args>
-cudaError_t launch_grouped(Kernel kernel, bool (&configured)[kMaxDevices], int pairs, int threads, int smem, cudaStream_t stream,
+cudaError_t launch_grouped(Kernel kernel, std::atomic<bool> (&configured)[kMaxDevices], int pairs, int threads, int smem, cudaStream_t stream,
                            const Args&... args) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
+    if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
   }
   return launch_pdl(kernel, dim3(2 * pairs), dim3(threads), smem, stream, args...);
 }
 template <bool kBf16, bool kMn>
 cudaError_t launch_rows(const CUtensorMap& w, const RowMaps& x, const GroupedParams& p, int pairs, cudaStream_t stream) {
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices] = {};
   return launch_grouped(fmoe_grouped_rows_kernel<kBf16, kMn>, configured, pairs, kGrpThreads, kGrpSmemBytes, stream, w, x, p);
 }
 template <bool kBf16>
 cudaError_t launch_wgrad(const CUtensorMap& dy, const CUtensorMap& x, const CUtensorMap& dw, const GroupedParams& p, int pairs,
                          cudaStream_t stream) {
-  static bool configured[kMaxDevices] = {false};
+  static std::atomic<bool> configured[kMaxDevices] = {};
   return launch_grouped(fmoe_grouped_wgrad_kernel<kBf16>, configured, pairs, kWgThreads, kWgSmemBytes, stream, dy, x, dw, p);
 }
 
