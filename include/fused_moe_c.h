@@ -430,6 +430,17 @@ FMOE_API int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const int3
 FMOE_API int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
                                   int32_t n, int32_t k, int32_t quant, void* out, int32_t* status, void* stream);
 
+/* What fmoe_matmul_block128 runs on for these sizes on the current device (m = 0: nothing, all zeros). */
+enum fmoe_matmul_kernel { FMOE_MATMUL_FEW_ROWS = 1, FMOE_MATMUL_TILES = 2, FMOE_MATMUL_CTA_PAIRS = 3 };
+typedef struct fmoe_matmul_info_c {
+  int32_t kernel;         /* fmoe_matmul_kernel */
+  int32_t rows_per_tile;  /* activation rows */
+  int32_t cols_per_tile;  /* weight rows */
+  int32_t k_split;        /* CTAs that share a tile's blocks of k (FMOE_MATMUL_FEW_ROWS) */
+  int32_t reserved[4];
+} fmoe_matmul_info_c;
+FMOE_API int fmoe_describe_matmul_block128(int64_t m, int32_t n, int32_t k, int32_t quant, fmoe_matmul_info_c* info);
+
 /* The gated activation: out[r, i] = row_weight[r] * SiLU(gu[r, i]) * gu[r, width + i], gu [rows,
  * 2*width] of dtype FMOE_BF16 or FMOE_F16 (gate columns, then up columns: the order of W1's rows),
  * row_weight f32 [rows] or NULL (1).  f32 arithmetic, one rounding.  width is a multiple of 8. */

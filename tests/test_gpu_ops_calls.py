@@ -253,3 +253,66 @@ print("same")
 """
     r = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+# ----------------------------------------------------------------------------- every kernel, and exact sums
+FORMS = {("few_rows", rows, split) for rows in (16, 32, 128) for split in (1, 2, 4, 8)} | {("tiles", 128, 1), ("cta_pairs", 256, 1)}
+
+
+def _whole(gen, limit, *shape):
+    return torch.randint(-limit, limit + 1, shape, device=DEV, generator=gen)
+
+
+def _exact_block(m, n, k, quant, seed):
+    """Whole numbers up to 2 with scales of 1/2, 1 and 2: multiples of 1/4 below 2^17, so every 32-bit sum is
+    exact in any order and the result is the reference rounded once."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed)
+    blocks, nb = k // 128, (n + 127) // 128
+    a, w = _whole(gen, 2, m, k).float(), _whole(gen, 2, n, k).float()
+    ea, ew = _whole(gen, 1, m, blocks), _whole(gen, 1, nb, blocks)
+    sa = torch.exp2(ea.float()) if quant == "block128" else torch.nn.functional.pad((ea + 127).to(torch.uint8), (0, -blocks % 4), value=255)
+    sw = torch.exp2(ew.float())
+    out = M.matmul_block128(a.to(torch.float8_e4m3fn), sa.contiguous(), w.to(torch.float8_e4m3fn), sw, quant)
+    ref = (a.double() * torch.exp2(ea.double()).repeat_interleave(128, 1)) @ (w.double() * sw.double().repeat_interleave(128, 1).repeat_interleave(128, 0)[:n]).T
+    assert torch.equal(out, ref.bfloat16()), (m, n, k, float((out.double() - ref).abs().max()))
+
+
+@pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
+def test_every_form_of_the_product_is_run_and_exact(quant):
+    """Each kernel, tile and split that the library may choose, found by asking it, at its smallest size and
+    at one with odd sizes and many blocks of K."""
+    found = {}
+    for m in (1, 5, 16, 17, 33, 40, 65, 100, 130, 250, 300, 384, 520, 639, 1030, 2040, 4096, 7960):
+        for n in (63, 128, 200, 1100, 2303, 4999, 7743, 9000, 18431):
+            for k in (128, 384, 512, 1024, 1408, 2048, 2432, 3968, 5632, 7168, 7296):
+                d = M.describe_matmul_block128(m, n, k, quant)
+                assert d["cols_per_tile"] == (128 if d["kernel"] == "few_rows" else 256)
+                if m * n * k <= 6e10:
+                    found.setdefault((d["kernel"], d["rows_per_tile"], d["k_split"]), []).append((m * n * k, m, n, k))
+    # whole K to a 128-row tile always takes longer than a 128 x 256 tile whose MMAs apply the scales
+    assert set(found) == FORMS - ({("few_rows", 128, 1)} if quant == "block128_ue8m0" else set())
+    for sizes in found.values():
+        _, *smallest = min(sizes)
+        _, *odd = max(s for s in sizes if s[0] <= max(4e9, min(sizes)[0]))
+        for m, n, k in {tuple(smallest), tuple(odd)}:
+            _exact_block(m, n, k, quant, seed=m + n + k)
+    assert M.operator_status(DEV) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,n,k", [([3, 0, 40], 136, 7168), ([300, 1], 7168, 72), ([2100, 4000], 264, 200)])
+def test_long_sums_of_the_grouped_products_are_exact(sizes, n, k, dtype):
+    """Whole numbers up to 2: every sum of a few thousand products is exact in 32 bits, so each result is the
+    reference rounded once."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(n)
+    rows, off = sum(sizes), offsets_of(sizes)
+    x, w, dy = (_whole(gen, 2, *s).to(dtype) for s in ((rows, k), (len(sizes), n, k), (rows, n)))
+    y, dx, dw = M.grouped_matmul(x, w, off), M.grouped_matmul_dgrad(dy, w, off), M.grouped_matmul_wgrad(dy, x, off)
+    lo = 0
+    for g, size in enumerate(sizes):
+        at = slice(lo, lo + size)
+        xg, dg, wg = x[at].double(), dy[at].double(), w[g].double()
+        assert torch.equal(y[at], (xg @ wg.T).to(dtype)) and torch.equal(dx[at], (dg @ wg).to(dtype)) and torch.equal(dw[g], (dg.T @ xg).to(dtype))
+        lo += size

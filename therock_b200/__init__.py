@@ -8,9 +8,10 @@ from .api import (FusedMoeTraits, FusedMoeArgs, fused_moe, fused_moe_workspace_s
                   moe_sorting, sort_capacity, workspace_layout, launches_per_run, describe_run, lib, LIB_PATH,
                   FmoeError, route, quantise_rows)
 from .ops import (grouped_matmul, grouped_matmul_dgrad, grouped_matmul_wgrad, matmul_block128, silu_mul,  # noqa: F401
-                  silu_mul_backward, silu_mul_quantise, operator_status)
+                  silu_mul_backward, silu_mul_quantise, operator_status, describe_matmul_block128)
 
 __all__ = ["FusedMoeTraits", "FusedMoeArgs", "fused_moe", "fused_moe_workspace_size", "moe_sorting",
            "sort_capacity", "workspace_layout", "launches_per_run", "describe_run", "lib", "LIB_PATH", "FmoeError", "route",
            "quantise_rows", "grouped_matmul", "grouped_matmul_dgrad", "grouped_matmul_wgrad", "matmul_block128",
-           "silu_mul", "silu_mul_backward", "silu_mul_quantise", "operator_status"]
+           "silu_mul", "silu_mul_backward", "silu_mul_quantise", "operator_status",
+           "describe_matmul_block128"]

@@ -12,6 +12,7 @@ namespace fmoe {
 namespace {
 
 constexpr int kMaxDevices = 64;
+static_assert(kHwTileN == kBmmTileN, "one size of tile to report");
 
 CUresult byte_map(CUtensorMap* tm, const void* base, int64_t rows, int cols, int box_rows) {
   const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
@@ -92,6 +93,16 @@ int small_log_split(int nt, int tiles, int kb, const ClusterRoom& room) {
   return log_split;
 }
 
+// The room for clusters of the kernel with nt rows to a tile.
+template <bool kBytes>
+cudaError_t small_room(int nt, ClusterRoom* room) {
+  switch (nt) {
+    case 16: return small_kernel_room<16, kBytes>(room);
+    case 32: return small_kernel_room<32, kBytes>(room);
+    default: return small_kernel_room<128, kBytes>(room);
+  }
+}
+
 template <int kNT, bool kBytes>
 int run_small(const void* a, const void* w, BlockSmallParams p, int k, cudaStream_t stream) {
   using Cfg = BlockSmallCfg<kNT>;
@@ -103,8 +114,6 @@ int run_small(const void* a, const void* w, BlockSmallParams p, int k, cudaStrea
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
   p.t_tiles = (p.m + kNT - 1) / kNT;
   const int tiles = p.t_tiles * ((p.n + 127) / 128);
-  const int log_split = small_log_split(kNT, tiles, p.kb, room);
-  p.split = 1 << log_split;
   // A CTA alone on its SM takes the deep pipeline, two to an SM half of it each.
   const bool alone = tiles * p.split <= room.most[0] || Cfg::kTmemCols == 512;
   int stages = kBsMaxStages;
@@ -127,6 +136,12 @@ int run_small_nt(int nt, const void* a, const void* w, const BlockSmallParams& p
     default: return run_small<128, kBytes>(a, w, p, k, stream);
   }
 }
+
+// What a product runs on: the kernel, and for few rows the CTAs that share a tile's K blocks.
+struct MatmulChoice {
+  int kernel;      // kOneCta, kPairOfCtas, or the rows to a tile of the kernel for few rows
+  int split;
+};
 
 // The kernel that is estimated to be done first: the one for few rows (16, 32 or 128 rows to a tile), or
 // 128 x 256 tiles of a CTA (kOneCta), or 256 x 256 tiles of a pair of CTAs (kPairOfCtas).  An estimate
@@ -163,6 +178,31 @@ int choose_kernel(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom&
   return choice;
 }
 
+// For sizes that check_sizes has passed, on the current device.
+template <bool kHw>
+cudaError_t choose(int64_t m, int n, int kb, MatmulChoice* choice) {
+  ClusterRoom room;
+  cudaError_t e = small_room<kHw>(16, &room);
+  if (e != cudaSuccess) return e;
+  *choice = {choose_kernel(m, n, kb, kHw, device_sm_count(), room), 1};
+  if (choice->kernel == kOneCta || choice->kernel == kPairOfCtas) return cudaSuccess;
+  e = small_room<kHw>(choice->kernel, &room);
+  const int64_t tiles = (m + choice->kernel - 1) / choice->kernel * ((n + 127) / 128);
+  if (e == cudaSuccess) choice->split = 1 << small_log_split(choice->kernel, static_cast<int>(tiles), kb, room);
+  return e;
+}
+
+int check_sizes(const char* name, int64_t m, int32_t n, int32_t k, int32_t quant) {
+  if (quant != FMOE_QUANT_BLOCK128 && quant != FMOE_QUANT_BLOCK128_UE8M0)
+    return fail(FMOE_ERR_INVALID_ARG, "%s: quant must be a block mode", name);
+  if (m < 0 || n <= 0 || k <= 0)
+    return fail(FMOE_ERR_INVALID_ARG, "%s: bad dimensions (m=%lld n=%d k=%d)", name, (long long)m, n, k);
+  if (k % 128) return fail(FMOE_ERR_UNSUPPORTED, "%s: k must be a multiple of 128", name);
+  if (m > 0x7fffff00LL || (m / kBmmTileM + 1) * (n / kBmmTileN + 1) > 0x7fffffffLL)
+    return fail(FMOE_ERR_UNSUPPORTED, "%s: problem too large", name);
+  return FMOE_OK;
+}
+
 }  // namespace
 
 cudaError_t take_block_matmul_status(int32_t* code) {
@@ -182,13 +222,8 @@ cudaError_t set_block_matmul_wait_limit(int64_t cycles) {
 extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
                                     int32_t n, int32_t k, int32_t quant, void* out, int32_t* status, void* stream) {
   using namespace fmoe;
-  if (quant != FMOE_QUANT_BLOCK128 && quant != FMOE_QUANT_BLOCK128_UE8M0)
-    return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: quant must be a block mode");
-  if (m < 0 || n <= 0 || k <= 0)
-    return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: bad dimensions (m=%lld n=%d k=%d)", (long long)m, n, k);
-  if (k % 128) return fail(FMOE_ERR_UNSUPPORTED, "fmoe_matmul_block128: k must be a multiple of 128");
-  if (m > 0x7fffff00LL || (m / kBmmTileM + 1) * (n / kBmmTileN + 1) > 0x7fffffffLL)
-    return fail(FMOE_ERR_UNSUPPORTED, "fmoe_matmul_block128: problem too large");
+  const int checked = check_sizes("fmoe_matmul_block128", m, n, k, quant);
+  if (checked != FMOE_OK) return checked;
   if (m == 0) return FMOE_OK;
   if (!a || !a_scale || !w || !w_scale || !out)
     return fail(FMOE_ERR_INVALID_ARG, "fmoe_matmul_block128: a, a_scale, w, w_scale and out are required");
@@ -202,24 +237,24 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
   const int sms = device_sm_count();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool hw = quant == FMOE_QUANT_BLOCK128_UE8M0;
-  ClusterRoom room;
-  FMOE_CUDA((hw ? small_kernel_room<16, true>(&room) : small_kernel_room<16, false>(&room)));
-  const int choice = choose_kernel(m, n, k / 128, hw, sms, room);
-  if (choice != kOneCta && choice != kPairOfCtas) {
+  MatmulChoice choice;
+  FMOE_CUDA(hw ? choose<true>(m, n, k / 128, &choice) : choose<false>(m, n, k / 128, &choice));
+  if (choice.kernel != kOneCta && choice.kernel != kPairOfCtas) {
     BlockSmallParams p{};
     p.a_scale = a_scale;
     p.w_scale = w_scale;
     p.m = static_cast<int>(m);
     p.n = n;
     p.kb = k / 128;
+    p.split = choice.split;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.status = status;
-    return hw ? run_small_nt<true>(choice, a, w, p, k, s) : run_small_nt<false>(choice, a, w, p, k, s);
+    return hw ? run_small_nt<true>(choice.kernel, a, w, p, k, s) : run_small_nt<false>(choice.kernel, a, w, p, k, s);
   }
   CUtensorMap ta, tw;
   CUresult r = byte_map(&ta, a, m, k, kBmmTileM);
   const int tile_n = hw ? kHwTileN : kBmmTileN;
-  const bool pair = choice == kPairOfCtas;
+  const bool pair = choice.kernel == kPairOfCtas;
   if (r == CUDA_SUCCESS) r = byte_map(&tw, w, n, k, !pair ? tile_n : hw ? HwCfg<true>::kWRows : BmmCfg<true>::kHalfRows);
   if (r != CUDA_SUCCESS) return fail(FMOE_ERR_CUDA, "fmoe_matmul_block128: tensor map (driver code %d)", static_cast<int>(r));
   BlockMatmulParams p{};
@@ -242,6 +277,28 @@ extern "C" int fmoe_matmul_block128(const void* a, const void* a_scale, const vo
     const int grid = tiles < sms ? tiles : sms;
     FMOE_CUDA(hw ? launch_hw<false>(ta, tw, p, grid, s) : launch_f32<false>(ta, tw, p, grid, s));
   }
+  return FMOE_OK;
+}
+
+extern "C" int fmoe_describe_matmul_block128(int64_t m, int32_t n, int32_t k, int32_t quant, fmoe_matmul_info_c* info) {
+  using namespace fmoe;
+  if (!info) return fail(FMOE_ERR_INVALID_ARG, "fmoe_describe_matmul_block128: info is required");
+  *info = fmoe_matmul_info_c{};
+  const int rc = check_sizes("fmoe_describe_matmul_block128", m, n, k, quant);
+  if (rc != FMOE_OK || m == 0) return rc;
+  MatmulChoice choice;
+  FMOE_CUDA(quant == FMOE_QUANT_BLOCK128_UE8M0 ? choose<true>(m, n, k / 128, &choice) : choose<false>(m, n, k / 128, &choice));
+  if (choice.kernel == kOneCta || choice.kernel == kPairOfCtas) {
+    const bool pair = choice.kernel == kPairOfCtas;
+    info->kernel = pair ? FMOE_MATMUL_CTA_PAIRS : FMOE_MATMUL_TILES;
+    info->rows_per_tile = pair ? 2 * kBmmTileM : kBmmTileM;
+    info->cols_per_tile = kBmmTileN;
+  } else {
+    info->kernel = FMOE_MATMUL_FEW_ROWS;
+    info->rows_per_tile = choice.kernel;
+    info->cols_per_tile = 128;
+  }
+  info->k_split = choice.split;
   return FMOE_OK;
 }
 

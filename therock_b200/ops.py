@@ -38,6 +38,7 @@ def _bound():
         l.fmoe_operator_status.argtypes = [i32, ctypes.POINTER(i32)]
         l.fmoe_grouped_matmul_wgrad.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, vp]
         l.fmoe_matmul_block128.argtypes = [vp, vp, vp, vp, i64, i32, i32, i32, vp, vp, vp]
+        l.fmoe_describe_matmul_block128.argtypes = [i64, i32, i32, i32, ctypes.POINTER(_MatmulInfo)]
         l.fmoe_silu_mul.argtypes = [vp, vp, i64, i32, i32, vp, vp]
         l.fmoe_silu_mul_quantise.argtypes = [vp, vp, i64, i32, i32, i32, vp, vp, vp]
         l.fmoe_silu_mul_backward.argtypes = [vp, vp, vp, i64, i32, i32, vp, vp, vp]
@@ -45,6 +46,12 @@ def _bound():
     return l
 
 
+class _MatmulInfo(ctypes.Structure):
+    _fields_ = [("kernel", ctypes.c_int32), ("rows_per_tile", ctypes.c_int32), ("cols_per_tile", ctypes.c_int32),
+                ("k_split", ctypes.c_int32), ("reserved", ctypes.c_int32 * 4)]
+
+
+_MATMUL_KERNEL = {0: "none", 1: "few_rows", 2: "tiles", 3: "cta_pairs"}
 _binding = None
 
 
@@ -288,6 +295,17 @@ def matmul_block128(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     _check(_bound().fmoe_matmul_block128(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), m, n, k,
                                          QUANT[quant], y.data_ptr(), None, _stream_of(a, stream)))
     return _filled(out, y)
+
+
+def describe_matmul_block128(m: int, n: int, k: int, quant: str = "block128") -> dict:
+    """What matmul_block128 runs on for these sizes on the current device: the kernel ("few_rows", "tiles"
+    or "cta_pairs"), the rows and columns of its tiles, and how many CTAs share a tile's blocks of k."""
+    if quant not in _BLOCK_QUANT:
+        raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
+    _sizes(n, k)
+    info = _MatmulInfo()
+    _check(_bound().fmoe_describe_matmul_block128(m, n, k, QUANT[quant], ctypes.byref(info)))
+    return {"kernel": _MATMUL_KERNEL[info.kernel], **{f: int(getattr(info, f)) for f in ("rows_per_tile", "cols_per_tile", "k_split")}}
 
 
 # ----------------------------------------------------------------------------- the gated activation
