@@ -443,12 +443,16 @@ FMOE_API int fmoe_describe_matmul_block128(int64_t m, int32_t n, int32_t k, int3
 
 /* The gated activation: out[r, i] = row_weight[r] * SiLU(gu[r, i]) * gu[r, width + i], gu [rows,
  * 2*width] of dtype FMOE_BF16 or FMOE_F16 (gate columns, then up columns: the order of W1's rows),
- * row_weight f32 [rows] or NULL (1).  f32 arithmetic, one rounding.  width is a multiple of 8. */
+ * row_weight f32 [rows] or NULL (1).  f32 arithmetic, one rounding.  width is a multiple of 8.  A gate
+ * below -88.7 gives zero (its sigmoid is below the smallest normal f32 number). */
 FMOE_API int fmoe_silu_mul(const void* gu, const float* row_weight, int64_t rows, int32_t width, int32_t dtype, void* out,
                            void* stream);
 /* The same rounded to dtype and then quantised to e4m3 with 1x128 scales, bit for bit what
- * fmoe_quantise_rows makes of fmoe_silu_mul's bf16 result (quant: FMOE_QUANT_BLOCK128 or
- * FMOE_QUANT_BLOCK128_UE8M0; width a multiple of 128). */
+ * fmoe_quantise_rows makes of fmoe_silu_mul's bf16 result, and by the same rule of its f16 result
+ * (quant: FMOE_QUANT_BLOCK128 or FMOE_QUANT_BLOCK128_UE8M0; width a multiple of 128).  A result that is
+ * infinite in dtype (f16: above 65504) makes its group's f32 scale infinite and the group's values NaN or
+ * zero; the power-of-two scale stays at 2^127.  At the other end, a group whose largest magnitude is not
+ * zero but below 448 * 2^-128 (1.3e-36) has an f32 scale without a finite reciprocal, with NaN for its zeros. */
 FMOE_API int fmoe_silu_mul_quantise(const void* gu, const float* row_weight, int64_t rows, int32_t width, int32_t dtype,
                                     int32_t quant, void* q, void* scales, void* stream);
 /* Gradients of fmoe_silu_mul: dgu [rows, 2*width] and, with row_weight, dweight f32 [rows]. */

@@ -316,3 +316,51 @@ def test_long_sums_of_the_grouped_products_are_exact(sizes, n, k, dtype):
         xg, dg, wg = x[at].double(), dy[at].double(), w[g].double()
         assert torch.equal(y[at], (xg @ wg.T).to(dtype)) and torch.equal(dx[at], (dg @ wg).to(dtype)) and torch.equal(dw[g], (dg.T @ xg).to(dtype))
         lo += size
+
+
+# ----------------------------------------------------------------------------- the quantising form from float16
+def _quantised(y, quant):
+    """e4m3 bytes and scales of y's groups of 128 by the rule of quantise_rows: absmax / 448 (1 for zeros), or
+    the smallest power of two that is no less; the reciprocal rounded once.  (A tensor divided by a number is
+    a product with its reciprocal on the GPU; 64 bits round a quotient of 32-bit numbers as one division does.)"""
+    v = y.float().view(y.shape[0], -1, 128)
+    amax = v.abs().amax(2)
+    s = torch.where(amax > 0, (amax.double() / 448).float(), torch.ones_like(amax))
+    if quant == "block128_ue8m0":
+        m, e = torch.frexp(s)
+        s = torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e))
+    return (v * (1 / s.double()).float()[:, :, None]).view(y.shape).to(torch.float8_e4m3fn), s
+
+
+@pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("rows,width", [(1, 128), (5, 384), (300, 1152), (16, 14336)])
+def test_silu_mul_quantise_of_float16(rows, width, weighted, quant):
+    """Rounded to float16 first, then quantised: bytes and scales of the rule applied to silu_mul's result."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(rows + width)
+    gu = (torch.randn(rows, 2 * width, device=DEV, generator=gen) * 3).half()
+    gu[rows // 2] = 0
+    weight = torch.rand(rows, device=DEV, generator=gen) if weighted else None
+    q, s = M.silu_mul_quantise(gu, quant, weight)
+    want_q, want_s = _quantised(M.silu_mul(gu, weight), quant)
+    groups = width // 128
+    got_s = s.view(torch.float32) if quant == "block128" else torch.exp2(s[:, :groups].float() - 127)
+    assert torch.equal(got_s, want_s) and torch.equal(q, want_q.view(torch.uint8))
+
+
+@pytest.mark.parametrize("quant", ["block128", "block128_ue8m0"])
+def test_a_group_that_overflows_float16_leaves_the_others_alone(quant):
+    """Above 65504 float16 is infinite, and so is its group's f32 scale; a power-of-two scale stays at its largest."""
+    gu = torch.ones(3, 768, device=DEV).half()
+    want_q, want_s = M.silu_mul_quantise(gu, quant)
+    gu[1, 130], gu[1, 384 + 130] = 300.0, 300.0
+    assert bool(torch.isinf(M.silu_mul(gu)[1, 130]))
+    q, s = M.silu_mul_quantise(gu, quant)
+    rest = torch.ones_like(q, dtype=torch.bool)
+    rest[1, 128:256] = False
+    assert torch.equal(q[rest], want_q[rest])
+    if quant == "block128":
+        s, want_s = s.view(torch.float32), want_s.view(torch.float32)
+    assert torch.equal(s[[0, 2], :3], want_s[[0, 2], :3]) and torch.equal(s[1, [0, 2]], want_s[1, [0, 2]])
+    assert bool(torch.isinf(s[1, 1])) if quant == "block128" else int(s[1, 1]) == 254
