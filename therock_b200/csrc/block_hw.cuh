@@ -285,7 +285,6 @@ fmoe_matmul_block128_hw_kernel(const __grid_constant__ CUtensorMap tm_a, const _
     if (!ok && threadIdx.x == 128) bmm_fail<kPair>(p.status, abort_flag, 0x24);
   }
 
-  __syncwarp();
   ptx::tc_fence_before();
   if (kPair) ptx::cluster_sync_all();      // neither CTA leaves while its partner can still signal it or read its shared memory
   else __syncthreads();

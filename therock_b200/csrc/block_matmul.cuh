@@ -90,7 +90,7 @@ static __device__ int g_bmm_status;      // for calls without a status word
 
 // kPair: both CTAs of a pair give up.
 template <bool kPair>
-__device__ __forceinline__ void bmm_fail(int* status, volatile int* abort_flag, int code) {
+__device__ __noinline__ void bmm_fail(int* status, volatile int* abort_flag, int code) {
   atomicExch(status != nullptr ? status : &g_bmm_status, kStatusBmmTimeout | code);
   if (kPair) ptx::raise_in_peer(abort_flag);
 }
@@ -410,7 +410,6 @@ fmoe_matmul_block128_kernel(const __grid_constant__ CUtensorMap tm_a, const __gr
     if (!ok && threadIdx.x == 256) bmm_fail<kPair>(p.status, abort_flag, 0x04);
   }
 
-  __syncwarp();
   ptx::tc_fence_before();
   if (kPair) ptx::cluster_sync_all();      // neither CTA leaves while its partner can still signal it or read its shared memory
   else __syncthreads();

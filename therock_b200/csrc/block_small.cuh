@@ -344,7 +344,6 @@ fmoe_matmul_block128_small_kernel(const __grid_constant__ CUtensorMap tm_a, cons
     }
   }
 
-  __syncwarp();
   ptx::tc_fence_before();
   __syncthreads();
   ptx::settle(abort_flag);

@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 
 static __device__ int g_grouped_status;      // for calls without a status word
 
-__device__ __forceinline__ void grouped_fail(const GroupedParams& p, volatile int* abort_flag, int code) {
-  atomicExch(p.status != nullptr ? p.status : &g_grouped_status, kStatusGroupedTimeout | code);
+static __device__ __noinline__ void grouped_fail(int* status, volatile int* abort_flag, int code) {
+  atomicExch(status != nullptr ? status : &g_grouped_status, kStatusGroupedTimeout | code);
   ptx::raise_in_peer(abort_flag);
 }
 
@@ -199,7 +199,6 @@ struct GroupedSmem {
 
 __device__ __forceinline__ void grouped_teardown(uint32_t tmem_base, int warp, const volatile int* abort_flag) {
   // neither CTA leaves while its partner can still signal its barriers or read its shared memory
-  __syncwarp();
   ptx::tc_fence_before();
   ptx::cluster_sync_all();
   ptx::settle(abort_flag);
@@ -275,7 +274,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
         if (++stage == kGrpStages) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) grouped_fail(p, s.abort_flag, 0x01);
+    if (!ok && lane == 0) grouped_fail(p.status, s.abort_flag, 0x01);
     ptx::pdl_release();   // all operands requested: the next kernel may begin its set-up
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (rank 0 only)
@@ -325,7 +324,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
         __syncwarp();
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok && lane == 0) grouped_fail(p, s.abort_flag, 0x02);
+      if (!ok && lane == 0) grouped_fail(p.status, s.abort_flag, 0x02);
     }
   } else {
     // ------------------------------------------------------------------ epilogue warps (both ranks)
@@ -380,7 +379,7 @@ fmoe_grouped_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
       if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
-    if (!ok && threadIdx.x == 64) grouped_fail(p, s.abort_flag, 0x03);
+    if (!ok && threadIdx.x == 64) grouped_fail(p.status, s.abort_flag, 0x03);
     // rows of no group: in front of the first one and behind the last
     const int head = s.starts[0], tail = s.starts[p.groups];
     const int vecs = p.n >> 3;
@@ -463,7 +462,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
         if (++stage == kWgStages) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) grouped_fail(p, s.abort_flag, 0x11);
+    if (!ok && lane == 0) grouped_fail(p.status, s.abort_flag, 0x11);
     ptx::pdl_release();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (rank 0 only)
@@ -511,7 +510,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
         __syncwarp();
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if (!ok && lane == 0) grouped_fail(p, s.abort_flag, 0x12);
+      if (!ok && lane == 0) grouped_fail(p.status, s.abort_flag, 0x12);
     }
   } else if (warp == 6) {
     // ------------------------------------------------------------------ ragged last stages (both ranks)
@@ -549,7 +548,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       __syncwarp();
       phases ^= 1u << last_stage;
     }
-    if (!ok && lane == 0) grouped_fail(p, s.abort_flag, 0x14);
+    if (!ok && lane == 0) grouped_fail(p.status, s.abort_flag, 0x14);
   } else {
     // ------------------------------------------------------------------ epilogue warps (both ranks)
     // Lane = row n of the tile.  64 columns at a time are rounded, written to the warp's buffer in the
@@ -611,7 +610,7 @@ fmoe_grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tm_dy, const __gri
       if (lane == 0) ptx::mbar_arrive_cluster_relaxed(ptx::map_to_rank(ptx::smem_u32(&s.acc_empty_bar[acc]), 0));
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
-    if (!ok && threadIdx.x == 64) grouped_fail(p, s.abort_flag, 0x13);
+    if (!ok && threadIdx.x == 64) grouped_fail(p.status, s.abort_flag, 0x13);
     if (lane == 0) ptx::bulk_wait<0>();
     __syncwarp();
   }

@@ -122,11 +122,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // that (loads into shared memory, MMAs on it and their commits) takes microseconds, and a CTA that left
 // earlier would have it land in its successor's memory.  So it stays for about a millisecond.
 constexpr long long kSettleCycles = 2000000LL;
+static __device__ __noinline__ void stay() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < kSettleCycles) {}
+}
 __device__ __forceinline__ void settle(const volatile int* abort_flag) {
-  if (*abort_flag) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < kSettleCycles) {}
-  }
+  if (*abort_flag) stay();
 }
 
 // ----------------------------------------------------------------------------- TMA
