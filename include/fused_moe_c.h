@@ -426,7 +426,8 @@ FMOE_API int fmoe_grouped_matmul_wgrad(const void* dy, const void* x, const int3
  * [m, k/128]; FMOE_QUANT_BLOCK128_UE8M0: bytes [m, roundup(k/128, 4)]), w [n, k], w_scale f32
  * [ceil(n/128), k/128] (powers of two for FMOE_QUANT_BLOCK128_UE8M0: only the exponent is read), out
  * bf16 [m, n].  k is a multiple of 128, m and n are any.  The kernel, and with it the order of the
- * f32 sums, depends on m, n and k. */
+ * f32 sums, depends on m, n and k.  A block's two scales are multiplied in f32: their product should be a
+ * normal number (2^-126 to 2^128), or the block loses digits or becomes infinite. */
 FMOE_API int fmoe_matmul_block128(const void* a, const void* a_scale, const void* w, const float* w_scale, int64_t m,
                                   int32_t n, int32_t k, int32_t quant, void* out, int32_t* status, void* stream);
 

@@ -16,8 +16,8 @@
 // What bounds a large product is power: a pair holds half of the weight rows in each CTA, which costs a
 // third less traffic from L2 and shared memory, and the tiles go through the result in bands.
 //
-// Measured on a B200, 8192 x 4096 x 7168: 163 us = 2950 TFLOP/s in a short run; back to back under the power
-// limit 194 us = 2480 TFLOP/s at 1250 MHz, as long as a library e4m3 product without block scales (195; one
+// Measured on a B200, 8192 x 4096 x 7168: 163 to 166 us = 2950 TFLOP/s in a short run; back to back under the power
+// limit 191 to 194 us = 2480 TFLOP/s at 1250 MHz, as long as a library e4m3 product without block scales (195; one
 // CTA to a tile 210, and without bands 218).
 #pragma once
 

@@ -146,13 +146,15 @@ struct MatmulChoice {
 // The kernel that is estimated to be done first: the one for few rows (16, 32 or 128 rows to a tile), or
 // 128 x 256 tiles of a CTA (kOneCta), or 256 x 256 tiles of a pair of CTAs (kPairOfCtas).  An estimate
 // is a fixed part (launch, set-up, the way of the first blocks, the result), with few rows one for each
-// halving of K over a cluster, and a time for each K block of the longest CTA, in nanoseconds, fitted to measured times of 1 to 2048 rows times weights of 1024 x 1024
-// up to 18432 x 7168; over those the choice between few rows and 128 x 256 is 1.1 % from the best on
-// average.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times as many at the same time;
-// with 128 rows there are whole rounds.  A pair starts 1.2 us later, but reads a third less from L2 and
-// shared memory, which under the power limit is a higher clock: 8192 x 4096 x 7168 takes 198 us instead of
-// 209 (power-of-two scales) and 241 instead of 253 (f32), 8192 x 1024 x 1024 12.2 instead of 11.6 and 16.1
-// instead of 14.8.
+// halving of K over a cluster, and a time for each K block of the longest CTA, in nanoseconds, fitted to
+// measured times of 1 to 2048 rows times weights of 1024 x 1024 up to 18432 x 7168; the constants for few rows
+// are those of f32 scales.  Over those sizes the choice between few rows and 128 x 256 is 1 % from the best
+// on average with f32 scales and about 2 % with power-of-two scales; the worst single one found is 32 x 7744
+// x 2048, 7.4 us where tiles of 16 rows take 5.7.  CTAs with 16 or 32 rows share an SM, which takes 1.6 times
+// as many at the same time; with 128 rows there are whole rounds.  A pair's constants rest on two shapes: it
+// starts 1.2 us later, but reads a third less from L2 and shared memory, which under the power limit is a
+// higher clock: 8192 x 4096 x 7168 takes 191 to 194 us instead of 210 (power-of-two scales) and 237 instead of
+// 253 (f32), 8192 x 1024 x 1024 12.2 instead of 11.6 and 16.1 instead of 14.8.
 enum : int { kOneCta = 0, kPairOfCtas = 1 };
 int choose_kernel(int64_t m, int n, int kb, bool hw, int sms, const ClusterRoom& room) {
   const int64_t n_tiles = (n + 127) / 128;

@@ -4,7 +4,7 @@
 //
 // The scales change with every block of K, so P_b is a fresh accumulator in tensor memory (one pipeline
 // stage: 128 elements of K) and eight epilogue warps add it, scaled, to running sums in registers:
-// acc += P_b * (sa * sw).  Warp (quadrant q, half h) owns row 32q + lane and columns 128h .. 128h + 127,
+// acc += P_b * (sa * sw), the product of the scales rounded to 32 bits.  Warp (quadrant q, half h) owns row 32q + lane and columns 128h .. 128h + 127,
 // one weight block.
 //
 // What bounds it is instructions and their latencies, not the MMAs (512 cycles a stage): issuing a
@@ -18,7 +18,7 @@
 // own 128 activation rows and half of the weight rows, so that a third less comes from L2 and the MMAs
 // read a third less of shared memory, and the tiles go through the result in bands.
 //
-// Measured on a B200, 8192 x 4096 x 7168: 201 us = 2393 TFLOP/s in a short run; back to back under the power
+// Measured on a B200, 8192 x 4096 x 7168: 201 to 205 us = 2390 TFLOP/s in a short run; back to back under the power
 // limit 237 us = 2030 TFLOP/s at 1410 MHz (one CTA to a tile: 212 and 253 at 1360 MHz; without bands 219 and
 // 260).  A library e4m3 product without block scales takes 195 us back to back.  In a short run and without
 // bands one issuing warp and one 256-column accumulator per stage took 245 us, sixteen epilogue warps of 64

@@ -7,8 +7,9 @@
 //                 group's rows
 //
 // Both are persistent kernels of CTA pairs (cta_group::2, 256 x 256 tiles, 64 elements of the
-// contraction per stage, six stages, two 256-column accumulators in tensor memory), with the roles
-// of the pair kernel of the fused operator: producer warp, MMA warp, four epilogue warps.
+// contraction per stage, six stages in the rows kernel and five in the wgrad kernel, two 256-column
+// accumulators in tensor memory), with the roles of the pair kernel of the fused operator: producer
+// warp, MMA warp, four epilogue warps.  A tile's contraction is one pair's, whatever its length.
 //
 // Rows kernel: the weights are the MMA's M side and the rows its N side.  M tiles of weights are
 // always full, and N goes in steps of 32, so a group of any size costs its own rows rounded up to
@@ -17,11 +18,13 @@
 // that nobody stores.
 //
 // Measured on a B200 (bf16; 1644 TFLOP/s and 6457 GB/s are what a library product and a copy reach there):
-//   8192 rows in 8 equal groups x 28672 x 4096: 1.21 ms = 1586 TFLOP/s in a short run, 1.36 ms under the
-//   power limit; 8192 rows in 32 equal groups x 4096 x 7168: y and dx 0.37 ms, 1290 TFLOP/s with the
-//   weights coming from memory at 5 TB/s (their loads alone take 0.31 ms, the MMAs alone 0.23); dw
-//   0.48 ms = 1010 TFLOP/s (loads, MMAs and the 1.9 GB of stores take 0.34 to 0.39 ms in any two of the
-//   three); 32 rows over 8 groups x 28672 x 4096: 0.295 ms = 6370 GB/s.
+//   8192 rows in 8 equal groups x 28672 x 4096: 1.21 to 1.33 ms = 1450 to 1586 TFLOP/s in a short run, 1.36 to
+//   1.50 under the power limit; 8192 rows in 32 equal groups x 4096 x 7168: y and dx 0.37 to 0.40 ms, 1200 to
+//   1290 TFLOP/s with the weights coming from memory at 5 TB/s (their loads alone take 0.31 ms, the MMAs
+//   alone 0.23), 0.49 under the power limit; dw 0.48 ms = 1010 TFLOP/s (loads, MMAs and the 1.9 GB of stores
+//   take 0.34 to 0.39 ms in any two of the three), 0.56 under the power limit; 31 groups of uneven sizes
+//   take 0.46, 0.46 and 0.56 ms, and 0.57, 0.56 and 0.64 under the power limit; 32 rows over 8 groups x 28672 x
+//   4096: 0.295 ms = 6370 GB/s; 2 rows through 1024 x 512: 4.85 us.
 // What it took: roles that run as whole warps with one elected thread (a lane-0 branch made the issue of
 // the MMAs and the loads the bound: 1.75 -> 1.31 ms), a store phase without a branch per store (-> 1.21), and
 // no cluster-scope release in a loop (dw 0.76 -> 0.49).  Prefetching the weights into L2 seven to sixteen

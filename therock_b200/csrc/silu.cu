@@ -6,8 +6,11 @@
 //
 // All of them are bound by memory: 6 bytes a cell forward (16-bit types), 10 backward, 5 with the
 // e4m3 result.  Every thread moves 16-byte vectors (8 cells) of the gate half and of the up half.
-// Measured on a B200, 16384 x 2048 bf16: forward 31 us = 6460 GB/s, the rate of a copy; backward with
-// row weights 53 us = 6340 GB/s (a block of 256 threads to a row, one vector each, took 63).
+// Measured on a B200, 16384 x 2048 bf16: forward 31 us = 6460 GB/s, the rate of a copy; backward 51 us =
+// 6600 GB/s, with row weights 53 to 56 us = 6000 to 6340 GB/s (a block of 256 threads to a row, one vector
+// each, took 63); to e4m3 36 us = 4650 GB/s with f32 scales and 37 with power-of-two scales (38 and 39 with row
+// weights), 8192 x 14336 126 and 130 us: the maximum of a group is a chain of four shuffles between the loads
+// and the stores, and the stores are half as wide.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -76,9 +79,11 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
                     Pair<T>::store(f[6], f[7]));
 }
 
-// 1 / (1 + exp(-g)) by the two special-function instructions (relative error below 2^-21 over the
-// range in which the result is not 0 or 1; the approximate reciprocal takes every finite input and
-// infinity, which the approximate division does not).
+// 1 / (1 + exp(-g)) by the two special-function instructions.  __expf is off by at most 2 + 1.173 |g| units
+// in the last place (2^-23), the sum and the reciprocal by one each, so the relative error is below
+// (4 + 1.173 |g|) 2^-23: 2^-20 up to |g| = 3, 2^-16 at -80, far inside a rounding to 16 bits.  Below -88.7
+// the exponential is infinite and the result zero (the approximate reciprocal takes every finite input
+// and infinity, which the approximate division does not).
 __device__ __forceinline__ float sigmoid(float g) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));

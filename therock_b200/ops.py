@@ -364,7 +364,8 @@ def silu_mul(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, out: O
 def silu_mul_quantise(gu: torch.Tensor, quant: str, row_weight: Optional[torch.Tensor] = None,
                       q: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, stream=None):
     """quantise_rows(silu_mul(gu, row_weight), quant) in one pass, bit for bit, for the block modes:
-    (q uint8 [rows, width], scales uint8 [rows, bytes]).  width is a multiple of 128.  No gradient."""
+    (q uint8 [rows, width], scales uint8 [rows, bytes]); from float16 by the same rule.  width is a multiple
+    of 128.  A result that is infinite in gu's type spoils its group of 128.  No gradient."""
     if quant not in _BLOCK_QUANT:
         raise FmoeError(-1, f"quant must be one of {_BLOCK_QUANT}")
     if q is None and scales is None and stream is None:
