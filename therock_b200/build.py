@@ -38,10 +38,11 @@ def build(force: bool = False, verbose: bool = False, checked: bool = False, tim
     while they are set), or with wait_limit_switch=True libfmoe_b200_waits.so (-DFMOE_WAIT_LIMIT_SWITCH:
     fmoe_set_wait_limit sets how long a wait in a kernel may take).  The variants never replace the
     product library."""
-    for on, suffix, define in ((checked, "checked", "-DFMOE_BOUNDS_CHECKS"), (timing_switches, "timing", "-DFMOE_TIMING_SWITCHES"),
-                               (wait_limit_switch, "waits", "-DFMOE_WAIT_LIMIT_SWITCH")):
-        if on:
-            return _build_variant(suffix, [define], force, verbose)
+    if checked or timing_switches:
+        return _build_variant("checked" if checked else "timing",
+                              ["-DFMOE_BOUNDS_CHECKS"] if checked else ["-DFMOE_TIMING_SWITCHES"], force, verbose)
+    if wait_limit_switch:      # the operators' kernels; the rest is the product library's
+        return _build_variant("waits", ["-DFMOE_WAIT_LIMIT_SWITCH"], force, verbose, only=("grouped.cu", "block_matmul.cu"))
     lib = _build_variant("", [], force, verbose)
     build_binding(force, verbose)
     return lib
@@ -94,14 +95,17 @@ def _recorded(path: str) -> str:
         return ""
 
 
-def _build_variant(suffix: str, defines: list, force: bool, verbose: bool) -> str:
+def _build_variant(suffix: str, defines: list, force: bool, verbose: bool, only=tuple(SOURCES)) -> str:
+    if set(only) != set(SOURCES):
+        _build_variant("", [], force, verbose)
+    product = globals()["OBJ_DIR"]
     OBJ_DIR = os.path.join(HERE, "build" + ("_" + suffix if suffix else ""))
     LIB = os.path.join(HERE, "libfmoe_b200" + ("_" + suffix if suffix else "") + ".so")
     NVCC_FLAGS = globals()["NVCC_FLAGS"] + defines
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
     jobs = []
-    for src in SOURCES:
+    for src in only:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ_DIR, src.replace(".cu", ".o"))
         if force or _stale(o, [s] + hdrs):
@@ -124,7 +128,7 @@ def _build_variant(suffix: str, defines: list, force: bool, verbose: bool) -> st
                 print(out)
             if rc != 0:
                 raise RuntimeError(f"nvcc failed for {cmd[-3]}")
-    objs = [os.path.join(OBJ_DIR, s.replace(".cu", ".o")) for s in SOURCES]
+    objs = [os.path.join(OBJ_DIR if s in only else product, s.replace(".cu", ".o")) for s in SOURCES]
     if force or jobs or _stale(LIB, objs):
         cmd = [_nvcc(), "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a"]
         r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
