@@ -188,6 +188,30 @@ def test_a_tracer_does_not_record_an_empty_result(name):
             program(x)
 
 
+@pytest.mark.parametrize("name", ["grouped", "silu"])
+def test_a_tracer_does_not_record_empty_gradients(name):
+    """The backward pass of a call that was made before the trace began."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, f, dy = _layer("M")
+    y = f(x, w) if name == "grouped" else M.silu_mul(x)
+    dy = dy if name == "grouped" else dy[:, :32].contiguous()
+    want = torch.autograd.grad(y, x, dy, retain_graph=True)[0]
+    with pytest.raises(RuntimeError, match="traced program"):
+        make_fx(lambda dy: torch.autograd.grad(y, x, dy, retain_graph=True)[0])(dy)
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+
+
+def test_gradients_with_offsets_and_weights_from_the_middle_of_a_tensor():
+    """Both need their types' alignment only, in the backward pass too."""
+    x, w, _, dy = _layer("M")
+    off = torch.cat([torch.full((1,), 7, dtype=torch.int32, device=DEV), offsets_of([10, 0, 23])])
+    rw = torch.rand(34, device=DEV)
+    for call, other in ((lambda o: torch.autograd.grad(M.grouped_matmul(x, w, o), (x, w), dy), off[1:]),
+                        (lambda o: torch.autograd.grad(M.silu_mul(x, o.detach().requires_grad_()), x, dy[:, :32].contiguous()), rw[1:])):
+        assert other.data_ptr() % 16
+        assert all(torch.equal(a, b) for a, b in zip(call(other), call(other.clone())))
+
+
 def test_traced_and_compiled_programs_hold_the_registered_operators():
     import therock_b200.torch_op  # noqa: F401
     from torch.fx.experimental.proxy_tensor import make_fx

@@ -75,6 +75,20 @@ void refuse_tangent(const at::Tensor& t) {
     throw Failure(FMOE_ERR_INVALID_ARG, "forward-mode derivatives are not supported");
 }
 
+// True while a tracer records what runs (make_fx, torch.jit.trace, export): it would see the allocation of
+// the result and nothing else.  Inside a registered operator, whose call it records, it is off.
+bool traced() {
+  auto on = [](at::DispatchKey k) { return c10::impl::tls_is_dispatch_key_included(k) && !c10::impl::tls_is_dispatch_key_excluded(k); };
+  return c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+         on(at::DispatchKey::Tracer) || on(at::DispatchKey::PreDispatch);
+}
+
+// A backward pass is traced as a call is: the recorded program would hold empty gradients.
+void refuse_traced_backward() {
+  if (traced())
+    throw Failure(FMOE_ERR_INVALID_ARG, "a traced program cannot hold this backward pass: use torch.ops.therock_b200 (import therock_b200.torch_op)");
+}
+
 // A backward pass that is being captured cannot hand gradients to a node of the default stream, which
 // cannot join a capture: a leaf has such a node as long as any earlier graph of it lives.  The engine
 // would break the capture, and with it the process; this ends the pass with an error instead.  It looks
@@ -105,9 +119,9 @@ void refuse_default_stream_in_capture(int device) {
 
 // A gradient that autograd may hand over with any strides, or a tensor that a hook on saved tensors gave
 // back, as the kernels read it.
-at::Tensor for_kernel(const at::Tensor& t) {
+at::Tensor for_kernel(const at::Tensor& t, uintptr_t to = 16) {
   at::Tensor c = t.contiguous();
-  return aligned(c, 16) ? c : c.clone();
+  return aligned(c, to) ? c : c.clone();
 }
 
 bool same_kind(const at::Tensor& a, const at::Tensor& b) { return a.scalar_type() == b.scalar_type() && a.get_device() == b.get_device(); }
@@ -154,11 +168,12 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    refuse_traced_backward();
     refuse_default_stream_in_capture(grads[0].get_device());
     torch::autograd::variable_list out(3);
     {
       at::NoGradGuard no_grad;
-      const at::Tensor dy = for_kernel(grads[0]), x = for_kernel(saved[0]), w = for_kernel(saved[1]), off = for_kernel(saved[2]);
+      const at::Tensor dy = for_kernel(grads[0]), x = for_kernel(saved[0]), w = for_kernel(saved[1]), off = for_kernel(saved[2], 4);
       if (!grouped_fits(x, w, off) || !same_kind(x, dy) || dy.size(0) != x.size(0) || dy.size(1) != w.size(1)) throw_not_saved();
       if (ctx->needs_input_grad(0)) out[0] = grouped(dy, w, off, true);
       if (ctx->needs_input_grad(1)) {
@@ -196,12 +211,13 @@ struct SiluMul : torch::autograd::Function<SiluMul> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    refuse_traced_backward();
     refuse_default_stream_in_capture(grads[0].get_device());
     torch::autograd::variable_list out(2);
     {
       at::NoGradGuard no_grad;
       const at::Tensor dy = for_kernel(grads[0]), gu = for_kernel(saved[0]);
-      const at::Tensor weight = saved[1].defined() ? for_kernel(saved[1]) : at::Tensor();
+      const at::Tensor weight = saved[1].defined() ? for_kernel(saved[1], 4) : at::Tensor();
       if (!silu_fits(gu, weight.defined() ? std::optional<at::Tensor>(weight) : std::nullopt) || !same_kind(gu, dy) ||
           dy.size(0) != gu.size(0) || 2 * dy.size(1) != gu.size(1))
         throw_not_saved();
@@ -226,14 +242,6 @@ PyObject* raise(const Failure& f) {
 }
 #define FMOE_TRY HANDLE_TH_ERRORS try {
 #define FMOE_CATCH } catch (const Failure& f) { return raise(f); } END_HANDLE_TH_ERRORS
-
-// True while a tracer records what runs (make_fx, torch.jit.trace, export): it would see the allocation of
-// the result and nothing else.  Inside a registered operator, whose call it records, it is off.
-bool traced() {
-  auto on = [](at::DispatchKey k) { return c10::impl::tls_is_dispatch_key_included(k) && !c10::impl::tls_is_dispatch_key_excluded(k); };
-  return c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
-         on(at::DispatchKey::Tracer) || on(at::DispatchKey::PreDispatch);
-}
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 

@@ -164,7 +164,7 @@ def _refuse_tracers() -> None:
 def _refuse_gradients(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise FmoeError(-1, "out and stream are for calls without gradients (use torch.no_grad or torch.cuda.stream)")
-    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise FmoeError(-1, "forward-mode derivatives are not supported")
 
 
