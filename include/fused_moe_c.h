@@ -411,7 +411,8 @@ FMOE_API int fmoe_operator_status(int32_t device, int32_t* status_out);
  * [0, rows], so any values are safe).  dtype: FMOE_BF16 or FMOE_F16; f32 sums, one rounding.
  *   transpose_w = 0: out[r, :] = w[g] x[r, :]      x [rows, k] -> out [rows, n]
  *   transpose_w = 1: out[r, :] = w[g]^T x[r, :]    x [rows, n] -> out [rows, k]  (gradient of x)
- * w is [groups, n, k].  Rows of no group are zero.  n and k are multiples of 8, groups <= 1024. */
+ * w is [groups, n, k].  Rows of no group are zero.  n and k are multiples of 8, groups <= 1024; sizes that a
+ * tile would carry past 32 bits are refused (rows above 0x7f000000, n or k above 0x7fffff00). */
 FMOE_API int fmoe_grouped_matmul(const void* x, const void* w, const int32_t* offsets, int64_t rows, int32_t groups,
                                  int32_t n, int32_t k, int32_t dtype, int32_t transpose_w, void* out, int32_t* status,
                                  void* stream);

@@ -200,7 +200,7 @@ int check_sizes(const char* name, int64_t m, int32_t n, int32_t k, int32_t quant
   if (m < 0 || n <= 0 || k <= 0)
     return fail(FMOE_ERR_INVALID_ARG, "%s: bad dimensions (m=%lld n=%d k=%d)", name, (long long)m, n, k);
   if (k % 128) return fail(FMOE_ERR_UNSUPPORTED, "%s: k must be a multiple of 128", name);
-  if (m > 0x7fffff00LL || (m / kBmmTileM + 1) * (n / kBmmTileN + 1) > 0x7fffffffLL)
+  if (m > 0x7fffff00LL || n > 0x7fffff00 || (m / kBmmTileM + 1) * (n / kBmmTileN + 1) > 0x7fffffffLL)
     return fail(FMOE_ERR_UNSUPPORTED, "%s: problem too large", name);
   return FMOE_OK;
 }

@@ -24,9 +24,10 @@ int check_grouped(const char* name, const int32_t* offsets, int64_t rows, int32_
   if (dtype != FMOE_BF16 && dtype != FMOE_F16) return fail(FMOE_ERR_UNSUPPORTED, "%s: bf16 and f16 only", name);
   if (groups > kGrpMaxGroups) return fail(FMOE_ERR_UNSUPPORTED, "%s: at most %d groups", name, kGrpMaxGroups);
   if (n % 8 || k % 8) return fail(FMOE_ERR_UNSUPPORTED, "%s: n and k must be multiples of 8", name);
-  // tile counts are 32-bit
+  // Row, column and tile numbers are 32-bit: a size plus a tile has to fit, and a group's rows plus the number of
+  // its pieces of 256.
   const int64_t wide = (n > k ? n : k) / kGrpTile + 1;
-  if (rows > 0x7fffff00LL || (rows / kGrpTile + groups + 1) * wide > 0x7fffffffLL ||
+  if (rows > 0x7f000000LL || n > 0x7fffff00 || k > 0x7fffff00 || (rows / kGrpTile + groups + 1) * wide > 0x7fffffffLL ||
       static_cast<int64_t>(groups) * (n / kGrpTile + 1) * (k / kGrpTile + 1) > 0x7fffffffLL)
     return fail(FMOE_ERR_UNSUPPORTED, "%s: problem too large", name);
   return FMOE_OK;
