@@ -388,3 +388,66 @@ def test_a_group_that_overflows_float16_leaves_the_others_alone(quant):
         s, want_s = s.view(torch.float32), want_s.view(torch.float32)
     assert torch.equal(s[[0, 2], :3], want_s[[0, 2], :3]) and torch.equal(s[1, [0, 2]], want_s[1, [0, 2]])
     assert bool(torch.isinf(s[1, 1])) if quant == "block128" else int(s[1, 1]) == 254
+
+
+# ----------------------------------------------------------------------------- ends of the ranges
+def test_no_rows_at_all():
+    """Empty results, zero gradients of the weights."""
+    x, gu = (torch.empty(0, c, device=DEV, dtype=torch.bfloat16).requires_grad_() for c in (64, 96))
+    w = torch.randn(3, 48, 64, device=DEV).bfloat16().requires_grad_()
+    rw = torch.empty(0, device=DEV).requires_grad_()
+    off = offsets_of([0, 0, 0])
+    y = M.grouped_matmul(x, w, off)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+    assert y.shape == (0, 48) and dx.shape == (0, 64) and dw.shape == w.shape and not bool(dw.any())
+    for weight in (None, rw):
+        z = M.silu_mul(gu, weight)
+        grads = torch.autograd.grad(z, [gu] + [weight] * (weight is not None), torch.empty_like(z))
+        assert z.shape == (0, 48) and [g.shape for g in grads] == [gu.shape] + [rw.shape] * (weight is not None)
+    q, s = M.silu_mul_quantise(torch.empty(0, 256, device=DEV).half(), "block128")
+    assert q.shape == (0, 128) and s.shape == (0, 4)
+    a, sa, b, sb = block_inputs(2, 70, 256, "block128", seed=1)
+    assert M.matmul_block128(a[:0], sa[:0], b, sb).shape == (0, 70)
+    assert M.operator_status(DEV) == 0
+
+
+def test_the_most_groups():
+    """1024 groups, most of them with a few rows, some with none, one with several pieces."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(9)
+    sizes = torch.randint(0, 9, (1024,), device=DEV, generator=gen)
+    sizes[0], sizes[511], sizes[1023] = 700, 0, 300
+    off = torch.cat([sizes.new_zeros(1), sizes.cumsum(0)]).int()
+    rows, n, k = int(off[-1]), 72, 136
+    x, w, dy = (_whole(gen, 2, *s).bfloat16() for s in ((rows, k), (1024, n, k), (rows, n)))
+    group = torch.repeat_interleave(torch.arange(1024, device=DEV), sizes)
+    y, dx, dw = M.grouped_matmul(x, w, off), M.grouped_matmul_dgrad(dy, w, off), M.grouped_matmul_wgrad(dy, x, off)
+    xd, wd, dd = x.double(), w.double(), dy.double()
+    assert torch.equal(y, torch.einsum("rk,rnk->rn", xd, wd[group]).bfloat16())
+    assert torch.equal(dx, torch.einsum("rn,rnk->rk", dd, wd[group]).bfloat16())
+    ref = torch.zeros(1024, n * k, device=DEV, dtype=torch.float64).index_add(0, group, (dd[:, :, None] * xd[:, None, :]).flatten(1))
+    assert torch.equal(dw, ref.view(1024, n, k).bfloat16())
+
+
+def test_an_activation_of_several_launches():
+    """A launch covers 2^30 vectors of 8; rows behind that are another launch's, with the same results as alone."""
+    rows, width = 8195, 1 << 20                                # 8192 rows are the first launch's
+    gu = torch.empty(rows, 2 * width, device=DEV, dtype=torch.bfloat16).normal_()
+    rw = torch.rand(rows, device=DEV)
+    spans = [slice(0, 2), slice(8190, 8192), slice(8192, rows)]
+    y = M.silu_mul(gu, rw)
+    for at in spans:
+        assert torch.equal(y[at], M.silu_mul(gu[at], rw[at].clone()))
+    for weight in (rw, None):
+        dgu, dw = M.silu_mul_backward(gu, y, weight)
+        for at in spans:
+            g, d = M.silu_mul_backward(gu[at], y[at], None if weight is None else weight[at].clone())
+            assert torch.equal(dgu[at], g) and (weight is None or torch.equal(dw[at], d))
+        del dgu, dw
+    del y
+    for quant in ("block128", "block128_ue8m0"):
+        q, s = M.silu_mul_quantise(gu, quant, rw)
+        for at in spans:
+            p, t = M.silu_mul_quantise(gu[at], quant, rw[at].clone())
+            assert torch.equal(q[at], p) and torch.equal(s[at], t)
+        del q, s
