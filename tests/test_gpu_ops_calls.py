@@ -188,6 +188,22 @@ def test_a_tracer_does_not_record_an_empty_result(name):
             program(x)
 
 
+TRANSFORMS = {"vmap": lambda f, x: torch.vmap(f)(x[None]), "functionalize": lambda f, x: torch.func.functionalize(f)(x),
+              "grad": lambda f, x: torch.func.grad(lambda t: f(t).float().sum())(x), "jvp": lambda f, x: torch.func.jvp(f, (x,), (x,))}
+
+
+@pytest.mark.parametrize("name,transform", [(n, t) for n in ("grouped", "silu", "quantise", "block") for t in TRANSFORMS
+                                            if n != "block" or t in ("vmap", "functionalize")])     # bytes have no derivatives
+def test_function_transforms_are_refused(name, transform):
+    off, w = offsets_of([10, 0, 23]), torch.randn(3, 96, 256, device=DEV).bfloat16()
+    a, sa, b, sb = block_inputs(33, 70, 256, "block128", seed=2)
+    x = a.view(torch.float8_e4m3fn).bfloat16()
+    f = {"grouped": lambda t: M.grouped_matmul(t, w, off), "silu": M.silu_mul, "quantise": lambda t: M.silu_mul_quantise(t, "block128")[0],
+         "block": lambda t: M.matmul_block128(t, sa, b, sb)}[name]
+    with pytest.raises(RuntimeError):
+        TRANSFORMS[transform](f, a.view(torch.uint8) if name == "block" else x)
+
+
 @pytest.mark.parametrize("name", ["grouped", "silu"])
 def test_a_tracer_does_not_record_empty_gradients(name):
     """The backward pass of a call that was made before the trace began."""

@@ -12,7 +12,8 @@ be captured in a CUDA graph (a forward and its backward pass in one graph; no ea
 same tensors that was recorded on the default stream may be alive).  Inputs are contiguous CUDA tensors on one device, which need not be
 the current one; a call on another stream than the current one allocates its results for that
 stream, and the caller orders the streams.  Bad arguments raise FmoeError before any launch, and so does a
-call that a tracer records (torch.ops.therock_b200 has the operators for traced and compiled programs)."""
+call that a tracer records (torch.ops.therock_b200 has all of them but silu_mul_quantise for traced and
+compiled programs)."""
 from __future__ import annotations
 
 import ctypes
@@ -158,7 +159,8 @@ def _refuse_tracers() -> None:
     call that fills it.  Inside a registered operator it is off."""
     if torch._C._get_dispatch_mode(_PROXY) is not None or any(
             torch._C._dispatch_tls_is_dispatch_key_included(k) and not torch._C._dispatch_tls_is_dispatch_key_excluded(k) for k in _TRACERS):
-        raise FmoeError(-1, "a traced program cannot hold this call: use torch.ops.therock_b200 (import therock_b200.torch_op)")
+        raise FmoeError(-1, "a traced program cannot hold this call: use the operator of torch.ops.therock_b200 (import "
+                            "therock_b200.torch_op), or leave the call out of the trace")
 
 
 def _refuse_gradients(*tensors) -> None:
